@@ -48,8 +48,17 @@ class Config(C.Structure):
     ]
 
 
+class PagePool(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("n_pages", C.c_int32), ("page_size", C.c_int32), ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32), ("format", C.c_int32),
+    ]
+
+
 # Every exported symbol of include/g4.h with its ctypes signature (restype, argtypes).
 _vp, _i32, _u64, _f = C.c_void_p, C.c_int32, C.c_uint64, C.c_float
+_i64, _poolp = C.c_int64, C.POINTER(PagePool)
 _i32p, _u64p, _fp = C.POINTER(C.c_int32), C.POINTER(C.c_uint64), C.POINTER(C.c_float)
 SIGNATURES = {
     "g4_last_error": (C.c_char_p, [_vp]),
@@ -105,6 +114,17 @@ SIGNATURES = {
     "g4_op_embed_gather": (C.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _f, _i32, _i32, _vp]),
     "g4_op_dense_bf16": (C.c_int, [_vp, _vp, _vp, _i32, _i32, _i32, _f, _vp]),
     "g4_op_softcap_argmax": (C.c_int, [_vp, _vp, _vp, _i32, _f, _vp]),
+    "g4_op_page_store": (C.c_int, [_poolp, _vp, _vp, _i32, _i64, _i64, _i32, _vp, _vp]),
+    "g4_op_page_read": (C.c_int, [_poolp, _vp, _i32, _i32, _vp, _vp, _i64, _i64, _vp]),
+    "g4_op_paged_attention": (C.c_int, [_poolp, _vp, _i64, _vp, _i64, _vp, _i32, _i32, _i32, _i32,
+                                        _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f, _vp, _u64,
+                                        _vp]),
+    "g4_op_paged_attention_workspace": (C.c_int, [_poolp, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+                                                  _u64p]),
+    "g4_op_verify_drafts": (C.c_int, [_vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _vp,
+                                      _vp, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _u64, _vp]),
+    "g4_op_verify_drafts_workspace": (C.c_int, [_i32, _i32, _i32, _i32, _u64p]),
+    "g4_op_paged_errors": (C.c_int, [_i32p]),
     "g4_op_math_probe": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _i32, _vp]),
 }
 

@@ -1,0 +1,387 @@
+// g4_drafts.cu -- verification of drafted tokens against the target model's probabilities.
+//
+// With x = logits / T a draft d stands when u w < p[d] = exp(x[d] - lse), lse = m + ln sum exp(x -
+// m): one pass over the row gives m and the sum. The token that follows is a race of exponential
+// clocks, argmax(ln weight + gumbel): with a certain drafter the weights of a refused row are p
+// without d, so ln weight is x itself up to a constant and the same pass over the row finds the
+// winner; no second pass and no cumulative sums, whose rounding would decide the token. Only a
+// drafter with probabilities needs the finished lse first (weights max(p - q, 0)): a second kernel
+// reads that one row of each sequence again.
+// Bound by HBM: the logits are read once.
+#include <cuda_runtime.h>
+#include <math.h>
+
+#include "g4_device.cuh"
+#include "g4_kernels.cuh"
+#include "g4_paged.cuh"
+
+namespace g4 {
+
+constexpr int kDraftThreads = 256;
+
+struct Race {
+  float key;
+  int idx;
+  // The greater key; the lower token on equal ones. A NaN key is never the greater one.
+  __device__ __forceinline__ void add(float k, int i) {
+    if (k > key || (k == key && i < idx)) {
+      key = k;
+      idx = i;
+    }
+  }
+};
+
+struct RowSum {
+  float m, s;
+  __device__ __forceinline__ void add(float om, float os) {
+    const float n = fmaxf(m, om);
+    const float ref = n == -INFINITY ? 0.0f : n;
+    s = s * expf(m - ref) + os * expf(om - ref);
+    m = n;
+  }
+};
+
+__device__ __forceinline__ DraftPart warp_join(DraftPart v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    const float om = __shfl_xor_sync(0xffffffffu, v.m, d), os = __shfl_xor_sync(0xffffffffu, v.s, d);
+    const float ok = __shfl_xor_sync(0xffffffffu, v.key, d);
+    const int oi = __shfl_xor_sync(0xffffffffu, v.idx, d);
+    RowSum r{v.m, v.s};
+    r.add(om, os);
+    Race c{v.key, v.idx};
+    c.add(ok, oi);
+    v = {r.m, r.s, c.key, c.idx};
+  }
+  return v;
+}
+// The block's sum; every thread of warp 0 receives it.
+__device__ __forceinline__ DraftPart block_join(DraftPart v, DraftPart *sh) {
+  v = warp_join(v);
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    v = threadIdx.x < kDraftThreads / 32 ? sh[threadIdx.x] : DraftPart{-INFINITY, 0.0f, -INFINITY, 0x7fffffff};
+    v = warp_join(v);
+  }
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ float logit_at(const DraftArgs &a, long long row, int t) {
+  const T *p = reinterpret_cast<const T *>(a.logits) + row * a.ld + t;
+  if constexpr (sizeof(T) == 4)
+    return *p;
+  else
+    return __bfloat162float(*p);
+}
+
+// VEC consecutive elements at p (aligned to VEC elements).
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T *p, float (&x)[VEC]) {
+  if constexpr (VEC == 1) {
+    if constexpr (sizeof(T) == 4)
+      x[0] = __ldg(p);
+    else
+      x[0] = __bfloat162float(*p);
+  } else if constexpr (sizeof(T) == 4) {
+    const float4 v = __ldg(reinterpret_cast<const float4 *>(p));
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+  } else {
+    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
+    x[0] = __uint_as_float(v.x << 16);
+    x[1] = __uint_as_float(v.x & 0xffff0000u);
+    x[2] = __uint_as_float(v.y << 16);
+    x[3] = __uint_as_float(v.y & 0xffff0000u);
+  }
+}
+
+struct SeqRows {
+  int row, n;
+};
+__device__ __forceinline__ SeqRows seq_rows(const DraftArgs &a, int b, bool report) {
+  const int b0 = a.row_begin[b], b1 = a.row_begin[b + 1];
+  SeqRows s;
+  s.row = min(max(b0, 0), a.rows);
+  const int end = min(max(b1, s.row), a.rows);
+  s.n = min(end - s.row, a.max_drafts + 1);
+  if (report && (b0 < 0 || b1 < b0 || b1 > a.rows || end - s.row > s.n)) paged_raise(a.err, G4_PAGED_BAD_LENGTH);
+  return s;
+}
+
+// What the scan leaves for the remainder's race: the row that emits (-1: done), its place and lse.
+struct DraftState {
+  int row, at;
+  float lse;
+  int pad;
+};
+
+// Block (split, j, b): split's share of sequence b's row j. The sequence's last block to finish
+// joins the shares and decides.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kDraftThreads) k_draft_scan(const DraftArgs a, DraftState *state) {
+  const int b = blockIdx.z, j = blockIdx.y, split = blockIdx.x, t = threadIdx.x;
+  const SeqRows sr = seq_rows(a, b, j == 0 && split == 0 && t == 0);
+  const int width = a.max_drafts + 1;
+  if (sr.n == 0) {
+    if (j == 0 && split == 0) {
+      for (int i = t; i < width; i += kDraftThreads) {
+        a.tokens[(long long)b * width + i] = -1;
+        a.logprobs[(long long)b * width + i] = 0.0f;
+      }
+      if (t == 0) {
+        a.counts[b] = 0;
+        state[b].row = -1;
+      }
+    }
+    return;
+  }
+  if (j >= sr.n) return;
+  __shared__ DraftPart sh[kDraftThreads / 32];
+  __shared__ bool last_block;
+  const float temp = a.temperature[b];
+  const bool greedy = temp == 0.0f, final_row = j == sr.n - 1;
+  const float inv = greedy ? 1.0f : __fdiv_rn(1.0f, temp);
+  const long long row = sr.row + j;
+  // A refused draft of a certain drafter is left out of its row's race; with probabilities the
+  // race of a drafted row is the second kernel's.
+  const int left_out = !greedy && !final_row && !a.probs ? a.drafts[row] : -1;
+  const bool race = greedy || final_row || !a.probs, noisy = race && !greedy;
+  const T *src = reinterpret_cast<const T *>(a.logits) + row * a.ld;
+  const float *noise = a.gumbel + (long long)b * a.ld_gumbel;
+  RowSum sum{-INFINITY, 0.0f};
+  Race best{-INFINITY, 0x7fffffff};
+  const int c1 = min(a.vocab, (split + 1) * a.chunk);
+  constexpr int U = 16 / VEC;   // loads in flight of each kind
+  for (int i0 = split * a.chunk + t * VEC; i0 < c1; i0 += kDraftThreads * VEC * U) {
+    float x[U][VEC], g[U][VEC];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int i = i0 + u * kDraftThreads * VEC;
+      if (i + VEC <= c1) {
+        load_vec<T, VEC>(src + i, x[u]);
+        if (noisy) load_vec<float, VEC>(noise + i, g[u]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+          x[u][e] = i + e < c1 ? logit_at<T>(a, row, i + e) : -INFINITY;
+          g[u][e] = noisy && i + e < c1 ? noise[i + e] : 0.0f;
+        }
+      }
+    }
+    float top = sum.m;
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int e = 0; e < VEC; e++) {
+        x[u][e] = __fmul_rn(x[u][e], inv);
+        top = fmaxf(top, x[u][e]);
+      }
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float s = sum.s * __expf(sum.m - ref);
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int e = 0; e < VEC; e++) {
+        s += __expf(x[u][e] - ref);
+        if (race) {
+          const int i = i0 + u * kDraftThreads * VEC + e;
+          const float key = noisy ? __fadd_rn(x[u][e], g[u][e]) : x[u][e];
+          if (key > best.key && i != left_out) best = {key, i};
+        }
+      }
+    sum = {top, s};
+  }
+  DraftPart v = block_join({sum.m, sum.s, best.key, best.idx}, sh);
+  DraftPart *parts = a.part + ((long long)b * width + j) * a.splits;
+  if (t == 0) {
+    parts[split] = v;
+    __threadfence();
+    last_block = atomicAdd(a.count + b, 1u) == (unsigned)(sr.n * a.splits) - 1;
+  }
+  __syncthreads();
+  if (!last_block) return;
+  __threadfence();
+
+  // Every row's sums, one warp a row; then the first draft that does not stand.
+  __shared__ float lse[kMaxDrafts + 1], lp[kMaxDrafts + 1];
+  __shared__ int chosen[kMaxDrafts + 1];
+  __shared__ bool stands[kMaxDrafts + 1];
+  const int warp = t >> 5, lane = t & 31;
+  for (int r = warp; r < sr.n; r += kDraftThreads / 32) {
+    const DraftPart *rp = a.part + ((long long)b * width + r) * a.splits;
+    DraftPart w{-INFINITY, 0.0f, -INFINITY, 0x7fffffff};
+    for (int s = lane; s < a.splits; s += 32) {
+      const float4 f = __ldcg(reinterpret_cast<const float4 *>(rp + s));
+      RowSum rs{w.m, w.s};
+      rs.add(f.x, f.y);
+      Race c{w.key, w.idx};
+      c.add(f.z, __float_as_int(f.w));
+      w = {rs.m, rs.s, c.key, c.idx};
+    }
+    w = warp_join(w);
+    if (lane == 0) {
+      const float ln = logf(w.s);
+      const int pick = w.idx == 0x7fffffff ? 0 : w.idx;
+      bool ok = false;
+      float lpd = 0.0f;
+      if (r < sr.n - 1) {
+        const int d = a.drafts[sr.row + r];
+        if (d >= 0 && d < a.vocab) {
+          lpd = (__fmul_rn(logit_at<T>(a, sr.row + r, d), inv) - w.m) - ln;
+          if (greedy) {
+            ok = d == pick;
+          } else {
+            const float q = a.probs ? a.probs[(sr.row + r) * a.ld_probs + d] : 1.0f;
+            ok = __fmul_rn(a.uniforms[sr.row + r], q) < expf(lpd);
+          }
+        }
+      }
+      stands[r] = ok;
+      chosen[r] = pick;
+      lp[r] = lpd;
+      lse[r] = w.m + ln;
+      // ln p of the row's winner, for the row that emits it.
+      if (!ok) lp[r] = (__fmul_rn(logit_at<T>(a, sr.row + r, pick), inv) - w.m) - ln;
+    }
+  }
+  __syncthreads();
+  __shared__ int stop;
+  if (t == 0) {
+    int r = 0;
+    while (r < sr.n - 1 && stands[r]) r++;
+    stop = r;
+    a.count[b] = 0;
+    a.counts[b] = r + 1;
+    const bool rest = a.probs && !greedy && r < sr.n - 1;
+    state[b] = {rest ? sr.row + r : -1, r, lse[r], 0};
+  }
+  __syncthreads();
+  for (int i = t; i < width; i += kDraftThreads) {
+    a.tokens[(long long)b * width + i] = i < stop ? a.drafts[sr.row + i] : (i == stop ? chosen[i] : -1);
+    a.logprobs[(long long)b * width + i] = i <= stop ? lp[i] : 0.0f;
+  }
+}
+
+// The remainder's race over the refused row of each sequence whose drafter gave probabilities:
+// ln max(p - q, 0) + gumbel, and x + gumbel for the case that no remainder is left.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kDraftThreads) k_draft_rest(const DraftArgs a, const DraftState *state) {
+  const int b = blockIdx.y, split = blockIdx.x, t = threadIdx.x;
+  const DraftState st = state[b];
+  if (st.row < 0) return;
+  __shared__ DraftPart sh[kDraftThreads / 32];
+  __shared__ bool last_block;
+  const float temp = a.temperature[b], inv = __fdiv_rn(1.0f, temp);
+  const T *src = reinterpret_cast<const T *>(a.logits) + (long long)st.row * a.ld;
+  const float *noise = a.gumbel + (long long)b * a.ld_gumbel;
+  const float *probs = a.probs + (long long)st.row * a.ld_probs;
+  // `s` and `m` carry the plain race here: its key, and its token as a float's bits.
+  Race rest{-INFINITY, 0x7fffffff}, plain{-INFINITY, 0x7fffffff};
+  const int c1 = min(a.vocab, (split + 1) * a.chunk);
+  constexpr int U = 8 / VEC;
+  for (int i0 = split * a.chunk + t * VEC; i0 < c1; i0 += kDraftThreads * VEC * U) {
+    float x[U][VEC], g[U][VEC], q[U][VEC];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int i = i0 + u * kDraftThreads * VEC;
+      if (i + VEC <= c1) {
+        load_vec<T, VEC>(src + i, x[u]);
+        load_vec<float, VEC>(noise + i, g[u]);
+        load_vec<float, VEC>(probs + i, q[u]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+          const bool in = i + e < c1;
+          x[u][e] = in ? logit_at<T>(a, st.row, i + e) : -INFINITY;
+          g[u][e] = in ? noise[i + e] : 0.0f;
+          q[u][e] = in ? probs[i + e] : 0.0f;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int e = 0; e < VEC; e++) {
+        const int i = i0 + u * kDraftThreads * VEC + e;
+        const float xs = __fmul_rn(x[u][e], inv);
+        const float left = __fsub_rn(expf(__fsub_rn(xs, st.lse)), q[u][e]);
+        if (left > 0.0f) {
+          const float key = __fadd_rn(logf(left), g[u][e]);
+          if (key > rest.key) rest = {key, i};
+        }
+        const float key = __fadd_rn(xs, g[u][e]);
+        if (key > plain.key) plain = {key, i};
+      }
+  }
+  const DraftPart r = block_join({-INFINITY, 0.0f, rest.key, rest.idx}, sh);
+  __syncthreads();
+  const DraftPart p = block_join({-INFINITY, 0.0f, plain.key, plain.idx}, sh);
+  DraftPart *parts = a.part + (long long)b * a.splits;
+  if (t == 0) {
+    parts[split] = {p.key, __int_as_float(p.idx), r.key, r.idx};
+    __threadfence();
+    last_block = atomicAdd(a.count + b, 1u) == (unsigned)a.splits - 1;
+  }
+  __syncthreads();
+  if (!last_block || t >= 32) return;
+  __threadfence();
+  rest = {-INFINITY, 0x7fffffff};
+  plain = {-INFINITY, 0x7fffffff};
+  for (int s = t; s < a.splits; s += 32) {
+    const float4 f = __ldcg(reinterpret_cast<const float4 *>(parts + s));
+    plain.add(f.x, __float_as_int(f.y));
+    rest.add(f.z, __float_as_int(f.w));
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    const float rk = __shfl_xor_sync(0xffffffffu, rest.key, d), pk = __shfl_xor_sync(0xffffffffu, plain.key, d);
+    const int ri = __shfl_xor_sync(0xffffffffu, rest.idx, d), pi = __shfl_xor_sync(0xffffffffu, plain.idx, d);
+    rest.add(rk, ri);
+    plain.add(pk, pi);
+  }
+  if (t == 0) {
+    const int pick = rest.idx != 0x7fffffff ? rest.idx : (plain.idx != 0x7fffffff ? plain.idx : 0);
+    const long long at = (long long)b * (a.max_drafts + 1) + st.at;
+    a.count[b] = 0;
+    a.tokens[at] = pick;
+    a.logprobs[at] = __fsub_rn(__fmul_rn(logit_at<T>(a, st.row, pick), inv), st.lse);
+  }
+}
+
+// Tokens a block scans: 16384, or fewer (in steps of 2048) until the rows fill the SMs twice.
+static int draft_chunk(int vocab, int rows) {
+  const int want = 2 * 148 / (rows > 0 ? rows : 1);
+  int splits = (vocab + 16383) / 16384;
+  if (splits < want) splits = want;
+  int chunk = (vocab + splits - 1) / splits;
+  return (chunk + 2047) / 2048 * 2048;
+}
+
+size_t verify_drafts_partials(int vocab, int rows, int batch, int max_drafts) {
+  const int chunk = draft_chunk(vocab, rows), splits = (vocab + chunk - 1) / chunk;
+  return (size_t)batch * (max_drafts + 1) * splits * sizeof(DraftPart) + (size_t)batch * sizeof(DraftState);
+}
+
+template <typename T, int VEC>
+static cudaError_t launch_drafts(const DraftArgs &a, DraftState *state, cudaStream_t st) {
+  const dim3 block(kDraftThreads);
+  cudaError_t e = launch_k(k_draft_scan<T, VEC>, dim3(a.splits, a.max_drafts + 1, a.batch), block, 0, st, false, a, state);
+  if (e == cudaSuccess && a.probs) e = launch_k(k_draft_rest<T, VEC>, dim3(a.splits, a.batch), block, 0, st, false, a, state);
+  return e;
+}
+
+cudaError_t launch_verify_drafts(const DraftArgs &args, cudaStream_t st) {
+  DraftArgs a = args;
+  a.chunk = draft_chunk(a.vocab, a.rows);
+  a.splits = (a.vocab + a.chunk - 1) / a.chunk;
+  DraftState *state = reinterpret_cast<DraftState *>(a.part + (size_t)a.batch * (a.max_drafts + 1) * a.splits);
+  // Four elements a load where every row starts on its boundary, else one.
+  const uintptr_t at = (uintptr_t)a.gumbel | (a.probs ? (uintptr_t)a.probs : 0);
+  const bool wide = a.ld % 4 == 0 && a.ld_gumbel % 4 == 0 && (!a.probs || a.ld_probs % 4 == 0) && !(at & 15) &&
+                    !((uintptr_t)a.logits & (a.type == G4_F32 ? 15 : 7));
+  if (a.type == G4_F32) return wide ? launch_drafts<float, 4>(a, state, st) : launch_drafts<float, 1>(a, state, st);
+  return wide ? launch_drafts<__nv_bfloat16, 4>(a, state, st) : launch_drafts<__nv_bfloat16, 1>(a, state, st);
+}
+
+}  // namespace g4

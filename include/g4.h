@@ -414,6 +414,128 @@ int g4_op_attention_noalloc(const float *q, const float *cache, float *out, int3
                             int32_t head_dim, int32_t q_count, int32_t q_start, int32_t kv_len,
                             int32_t window, int32_t max_context, void *stream);
 
+/* ------------------------------------------------------------- paged, quantised KV cache */
+/*
+ * Operators of a server that keeps its keys and values in pages shared by its sequences (no
+ * counterpart in the reference, whose cache is one contiguous f32 region, src/kv.ts:59-148). They
+ * are used in this order: g4_op_page_store quantises a step's new rows as it writes them,
+ * g4_op_paged_attention attends over the pages (decode tokens, verify passes and prefill chunks in
+ * one ragged batch), g4_op_verify_drafts decides which drafted tokens stand; g4_op_page_read takes
+ * rows back out. Everything is device memory of the current device, on the caller's stream;
+ * nothing is allocated and nothing is waited for.
+ *
+ * Element types of rows and logits:                                                            */
+#define G4_F32 0
+#define G4_BF16 1
+/* What a page holds: bf16 rows, or 8-bit codes with one f32 scale per (token, head). A value is
+ * code * scale; int8 codes lie in -127..127, e4m3 codes are finite (at most 448). */
+#define G4_PAGE_BF16 0
+#define G4_PAGE_INT8 1
+#define G4_PAGE_E4M3 2
+
+/*
+ * A pool of pages. k, v: [n_pages, kv_heads, page_size, head_dim]; k_scale, v_scale: f32
+ * [n_pages, kv_heads, page_size], NULL for bf16 pages; all 16-byte aligned. page_size is a
+ * multiple of 16 up to 1024, head_dim 64, 128, 256 or 512. A position of a page is named by its
+ * slot, page * page_size + offset; n_pages * page_size < 2^31.
+ */
+typedef struct g4_page_pool {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int32_t n_pages, page_size, kv_heads, head_dim;
+  int32_t format; /* G4_PAGE_* */
+} g4_page_pool;
+
+/*
+ * Store rows k, v [tokens, kv_heads, head_dim] (type; consecutive tokens k_stride / v_stride
+ * elements apart; rows 16-byte aligned) at slots[tokens] (int32, distinct). A negative slot skips
+ * its token, one past the pool skips it and raises G4_PAGED_BAD_PAGE. 8-bit pages, per (token, head):
+ *   scale = max|x| / 127 (int8) or / 448 (e4m3), in f32;
+ *   code = x / scale rounded to nearest even, in range; 0 where scale is 0.
+ * A row that holds a NaN or an infinity gets scale NaN and codes 0: all of it reads back as NaN.
+ * bf16 pages: each value rounded to nearest even.
+ */
+int g4_op_page_store(const g4_page_pool *pool, const void *k, const void *v, int32_t type,
+                     int64_t k_stride, int64_t v_stride, int32_t tokens, const int32_t *slots,
+                     void *stream);
+
+/*
+ * The rows at slots[tokens] back as k_out, v_out [tokens, kv_heads, head_dim] (type, strides as
+ * above): code * scale in f32, rounded once to the type. A negative slot gives zeros; one past the
+ * pool gives zeros and raises G4_PAGED_BAD_PAGE.
+ */
+int g4_op_page_read(const g4_page_pool *pool, const int32_t *slots, int32_t tokens, int32_t type,
+                    void *k_out, void *v_out, int64_t k_stride, int64_t v_stride, void *stream);
+
+/*
+ * Attention of new tokens over the pages. q, out: [rows, heads, head_dim] (type; consecutive rows
+ * q_stride / out_stride elements apart, 16-byte aligned); heads a multiple of kv_heads, query head
+ * h reads KV head h / (heads / kv_heads), heads / kv_heads at most 128. Sequence b of `batch` owns
+ * rows q_begin[b] .. q_begin[b + 1] - 1; its row i is the query at position q_pos[b] + i and sees
+ * the positions t <= q_pos[b] + i with t < kv_len[b] and, for window > 0, t > q_pos[b] + i -
+ * window (window 0: all; the window includes the query's own position). Position t lies in page
+ * page_table[b * table_stride + t / page_size]; entries of pages without a visible position are
+ * not read.
+ *   out = sum_t softmax_t(scale * q . k_t) v_t, lse = ln sum_t exp(scale * q . k_t)
+ * with lse f32 [rows, heads] or NULL. A row that sees nothing gets out 0 and lse -inf. Values at
+ * positions that a row does not see never reach it, whatever they are. max_q and max_kv bound the
+ * sequences' rows and kv_len: a longer sequence, rows past `rows` or positions past the page table
+ * are cut off there and raise G4_PAGED_BAD_LENGTH; a page outside the pool is left out and raises
+ * G4_PAGED_BAD_PAGE. Sums and softmax statistics are f32 and in a fixed order: results do not
+ * depend on the stream or on what else runs, but the split over a long context follows the batch's
+ * shape (batch, max_q, max_kv), so the last bits may differ between batches.
+ * workspace: g4_op_paged_attention_workspace bytes of device memory, 256-byte aligned, zeroed
+ * before its first use; each call leaves it ready for the next. Calls that share one must be in
+ * stream order.
+ */
+int g4_op_paged_attention(const g4_page_pool *pool, const void *q, int64_t q_stride, void *out,
+                          int64_t out_stride, float *lse, int32_t type, int32_t heads, int32_t rows,
+                          int32_t batch, const int32_t *q_begin, const int32_t *q_pos,
+                          const int32_t *kv_len, const int32_t *page_table, int32_t table_stride,
+                          int32_t max_q, int32_t max_kv, int32_t window, float scale,
+                          void *workspace, uint64_t workspace_bytes, void *stream);
+int g4_op_paged_attention_workspace(const g4_page_pool *pool, int32_t type, int32_t heads,
+                                    int32_t rows, int32_t batch, int32_t max_q, int32_t max_kv,
+                                    int32_t window, uint64_t *bytes);
+
+/*
+ * Verification of drafted tokens under sampling. Sequence b owns the rows row_begin[b] ..
+ * row_begin[b + 1] - 1 of logits [rows, vocab] (type, rows ld apart): every row but its last tests
+ * the drafted token drafts[row] (drafts: int32 [rows]), the last one follows them all. With
+ * x = logits * (1 / temperature[b]) and p = softmax(x):
+ *   a draft d of row r stands when uniforms[r] * w < p[d], w being draft_probs[r, d] (f32
+ *   [rows, vocab], rows ld_probs apart) or 1 where draft_probs is NULL (a drafter that is certain);
+ *   the first row whose draft does not stand emits argmax_t(ln max(p[t] - draft_probs[r, t], 0) +
+ *   gumbel[b, t]), or without draft_probs argmax_{t != d}(x[t] + gumbel[b, t]): a sample of the
+ *   normalised remainder max(p - w, 0) when gumbel (f32 [batch, vocab], rows ld_gumbel apart) holds standard
+ *   Gumbel numbers. Where rounding leaves no remainder, and in the last row, it is
+ *   argmax_t(x[t] + gumbel[b, t]), a sample of p.
+ * temperature 0 is greedy: x = logits, a draft stands when it is the argmax, and the emitted token
+ * is the argmax. Ties go to the lowest token; a NaN is never the greatest. Out per sequence:
+ * counts[b] tokens emitted (accepted drafts and the one chosen; 0 for a sequence without rows),
+ * tokens[b, 0 .. max_drafts] with -1 past them, and logprobs the same shape: ln p of each, 0 past
+ * them. A drafted token outside the vocabulary never stands. A sequence with more than max_drafts
+ * + 1 rows is cut off there and raises G4_PAGED_BAD_LENGTH. rows * vocab may pass 2^31.
+ * workspace as for attention.
+ */
+int g4_op_verify_drafts(const void *logits, int64_t ld, int32_t type, int32_t vocab, int32_t rows,
+                        int32_t batch, const int32_t *row_begin, const int32_t *drafts,
+                        const float *draft_probs, int64_t ld_probs, const float *uniforms,
+                        const float *gumbel, int64_t ld_gumbel, const float *temperature,
+                        int32_t max_drafts, int32_t *tokens, float *logprobs, int32_t *counts,
+                        void *workspace, uint64_t workspace_bytes, void *stream);
+int g4_op_verify_drafts_workspace(int32_t vocab, int32_t rows, int32_t batch, int32_t max_drafts,
+                                  uint64_t *bytes);
+
+/*
+ * What the operators above found wrong in device data since the last call, for the current device:
+ * an OR of the bits below, cleared by the call. Waits for the device.
+ */
+#define G4_PAGED_BAD_PAGE 1   /* a slot or a page id outside the pool */
+#define G4_PAGED_BAD_LENGTH 2 /* lengths past the bounds the call was given */
+#define G4_PAGED_TIMEOUT 4    /* a bounded device wait gave up; that call's output is not complete */
+int g4_op_paged_errors(int32_t *flags);
+
 /*
  * Failure detection without a fault (no counterpart in the reference, whose lost-device handling
  * is src/engine.ts:791-798). A one-thread kernel copies `bytes` (16..4096, a multiple of 16) from

@@ -347,8 +347,8 @@ int check_attention(const char *who, const g4_page_pool *pool, int32_t type, int
     return set_error(G4_ERR_INVALID, "%s: %d query heads over %d KV heads (a multiple, at most 128 times)", who, heads, a->pool.kv_heads);
   if (rows < 0 || batch < 0 || max_q < 0 || max_kv < 0 || window < 0)
     return set_error(G4_ERR_INVALID, "%s: rows %d, batch %d, max_q %d, max_kv %d, window %d", who, rows, batch, max_q, max_kv, window);
-  if (rows > (1 << 24) || batch > 65535 || max_kv > (1 << 30))
-    return set_error(G4_ERR_UNSUPPORTED, "%s: rows %d (at most 2^24), batch %d (65535), max_kv %d (2^30)", who, rows, batch, max_kv);
+  if ((long long)rows * heads >= (1ll << 30) || batch > 65535 || max_kv > (1 << 30))
+    return set_error(G4_ERR_UNSUPPORTED, "%s: rows %d x %d heads (fewer than 2^30), batch %d (at most 65535), max_kv %d (2^30)", who, rows, heads, batch, max_kv);
   a->type = type;
   a->heads = heads;
   a->group = heads / a->pool.kv_heads;

@@ -28,9 +28,10 @@ struct PagedAttn {
   const int32_t *q_begin, *q_pos, *kv_len, *table;
   int table_stride, max_q, max_kv, window;
   float scale;
-  // The split over the context (set by the launcher): tokens per split, splits per sequence, the
-  // per-split partials and the count of splits that have finished.
-  int split_tokens, splits;
+  // The split over the context (set by the launcher): tiles of 16 positions per split, splits per
+  // sequence, row groups per (sequence, KV head); the splits' partials and the counts of finished
+  // ones.
+  int split_tiles, splits, row_groups;
   float *part;
   uint32_t *count;
   int *err;
@@ -89,11 +90,11 @@ __device__ __forceinline__ SeqSpan seq_span(const PagedAttn &a, int b) {
     paged_raise(a.err, G4_PAGED_BAD_LENGTH);
   return s;
 }
-// The positions [lo, hi) that the row at position p sees.
+// The positions [lo, hi) that the row at position p sees: within 0 .. kv and neither end falling
+// as p grows, also where nothing is seen.
 __device__ __forceinline__ void row_range(const PagedAttn &a, int p, int kv, int &lo, int &hi) {
-  hi = min(p + 1, kv);
-  lo = a.window > 0 ? max(0, p - a.window + 1) : 0;
-  if (hi < lo) hi = lo;
+  hi = max(0, min(p + 1, kv));
+  lo = min(hi, a.window > 0 ? max(0, p - a.window + 1) : 0);
 }
 
 cudaError_t launch_paged_attention(const PagedAttn &a, cudaStream_t st);

@@ -1,4 +1,29 @@
-// g4_paged_attn.cu -- attention of new tokens over paged, quantised keys and values.
+// g4_paged_attn.cu -- attention of few new tokens (decode steps, verify passes) over paged,
+// quantised keys and values.
+//
+// For the rows (query, head) that share a KV head, with codes K, V and scales ks, vs per position:
+//   s_t = scale ks_t (q . K_t),  p_t = exp(s_t - M),  o = sum_t p_t vs_t V_t / sum_t p_t.
+// M is the running maximum of s_t + ln vs_t, not of s_t: the greatest p_t vs_t is then 1 and the
+// products' 16-bit weights keep their precision however far the scales lie apart; the sum of p_t
+// is f32. What bounds the kernel is reading the codes once from HBM (1 byte a value at 8 bits), so
+// everything else has to stay out of the loads' way:
+//  - Codes go from global memory straight into the registers of the matrix products, with no
+//    shared memory between. The sums over head_dim and over positions may run in any order, so
+//    each lane's 16-byte load is taken as it comes: for S^T = K Q^T (16 positions x 8 rows) lane
+//    (g, c) holds 16 codes of positions g and g + 8 as four K steps, for O^T = V^T P^T (16
+//    dimensions x 8 rows) 16 codes of positions 2c, 2c + 1, 2c + 8, 2c + 9, two dimensions a step.
+//    8-bit codes become f16 exactly in two instructions per pair or less; Q is laid out to match,
+//    in shared memory, once.
+//  - Eight rows fill the N of the products, so a group of 8 heads wastes none of it, and one
+//    8 x 8 transpose in registers turns S^T's layout into P^T's.
+//  - A ring of four 16-register buffers keeps up to three chunks of 2 KB a warp in flight through
+//    the score and the softmax of the chunk at hand.
+//  - f32 rows: q and p vs are carried in two f16 parts (8-bit codes; 22 bits together) or three
+//    bf16 parts (bf16 pages), one product each, all accumulated in f32.
+// The warps of a block take a split's tiles in turn and join through shared memory. A context that
+// one block per (sequence, KV head) would leave most SMs idle for is split over blocks; the
+// last of 16 splits to finish joins them, and the last such group joins the groups (one block
+// would read 2.4 MB alone for 148 splits of head_dim 512).
 #include <cuda_runtime.h>
 #include <math.h>
 
@@ -8,67 +33,723 @@
 
 namespace g4 {
 
-// One warp per (row, head), one position at a time, f32 throughout. With V = scale * code the
-// running maximum is that of score + ln(scale), so that the greatest weight p * scale of a row is
-// always 1, however far the scales lie apart.
-__device__ __forceinline__ float paged_code(const Pool &p, const uint8_t *base, long long row, int d) {
-  if (p.fmt == G4_PAGE_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(base)[row * p.hd + d]);
-  const uint8_t c = base[row * p.hd + d];
-  if (p.fmt == G4_PAGE_INT8) return (float)(int8_t)c;
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+constexpr int kDecWarps = 4;
+constexpr int kJoin = 16;            // partials one block joins
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+constexpr float kWeightBits = 14.0f; // 8-bit codes: weights are scaled by 2^14, clear of f16's subnormals
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// l 2^d for d <= 0. l may be as large as 2^114 (positions whose V scale is next to nothing), so that
+// 2^d alone could underflow where the product does not.
+__device__ __forceinline__ float rescale(float l, float d) {
+  const float h = ex2(0.5f * d);
+  return (l * h) * h;
+}
+template <bool HALF>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  if (HALF)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
+
+// Four codes in memory order as two f16 pairs. int8: u = code + 128 as the low byte of 1024 + u
+// (exponent bits 0x64), less 1152: exact. e4m3 values are f16 values.
+template <int FMT>
+__device__ __forceinline__ void codes4(uint32_t w, uint32_t &lo, uint32_t &hi) {
+  if (FMT == G4_PAGE_INT8) {
+    const uint32_t x = w ^ 0x80808080u, magic = 0x64646464u;
+    const uint32_t a = __byte_perm(x, magic, 0x4140), b = __byte_perm(x, magic, 0x4342);
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));   // 1152
+    lo = half2_bits(__hsub2(*reinterpret_cast<const __half2 *>(&a), off));
+    hi = half2_bits(__hsub2(*reinterpret_cast<const __half2 *>(&b), off));
+  } else {
+    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffff), __NV_E4M3);
+    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+    lo = *reinterpret_cast<const uint32_t *>(&a);
+    hi = *reinterpret_cast<const uint32_t *>(&b);
+  }
 }
 
-__global__ void __launch_bounds__(128) k_paged_attention(const PagedAttn a) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y;
-  const SeqSpan s = seq_span(a, b);
-  const long long item = (long long)blockIdx.x * 4 + warp;
-  const int i = (int)(item / a.heads), h = (int)(item % a.heads);
-  if (i >= s.n) return;
-  const Pool &p = a.pool;
-  const int kvh = h / a.group, hd = p.hd;
-  float q[16], o[16];
-  const long long qo = (long long)(s.row + i) * a.q_stride + (long long)h * hd;
-  for (int j = 0; j < hd / 32; j++) {
-    const int d = j * 32 + lane;
-    q[j] = a.type == G4_F32 ? ((const float *)a.q)[qo + d] : __bfloat162float(((const __nv_bfloat16 *)a.q)[qo + d]);
-    o[j] = 0.0f;
+// v as parts of HALF (f16) or bf16, greatest first; their sum is v to 11 NP (or 8 NP) bits.
+template <bool HALF, int NP>
+__device__ __forceinline__ void split2(float v0, float v1, uint32_t (&out)[NP]) {
+#pragma unroll
+  for (int i = 0; i < NP; i++) {
+    if (HALF) {
+      const __half2 h = __floats2half2_rn(v0, v1);
+      out[i] = half2_bits(h);
+      if (i + 1 < NP) {
+        const float2 f = __half22float2(h);
+        v0 = __fsub_rn(v0, f.x);
+        v1 = __fsub_rn(v1, f.y);
+      }
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v0, v1);
+      out[i] = *reinterpret_cast<const uint32_t *>(&h);
+      if (i + 1 < NP) {
+        v0 = __fsub_rn(v0, __low2float(h));
+        v1 = __fsub_rn(v1, __high2float(h));
+      }
+    }
   }
-  int lo, hi;
-  row_range(a, s.pos + i, s.kv, lo, hi);
-  float m = -INFINITY, l = 0.0f;
-  for (int t = lo; t < hi; t++) {
-    const int page = a.table[(long long)b * a.table_stride + t / p.page_size];
-    if (page < 0 || page >= p.n_pages) {
-      if (lane == 0) paged_raise(a.err, G4_PAGED_BAD_PAGE);
+}
+
+template <int FMT, int HD, int NP>
+struct DecShape {
+  static constexpr bool HALF = FMT != G4_PAGE_BF16;
+  static constexpr int ES = HALF ? 1 : 2;              // bytes of a code
+  static constexpr int ROW = HD * ES;                  // bytes of a position
+  static constexpr bool NARROW = ROW == 64;            // V loads of 8 bytes instead of 16
+  static constexpr int HC = NARROW ? 1 : ROW / 128;    // chunks of K, and of V, per tile
+  static constexpr int C = 2 * HC;
+  static constexpr int NB = 4;                         // ring buffers
+  static constexpr int TILES = C >= NB ? 1 : NB / C;   // tiles per pass of the unrolled loop
+  static constexpr int KSTEPS = HD / 16;
+  // Blocks per SM the registers are bounded for: O takes HD / 4 registers, the ring 64.
+  static constexpr int OCC = HD <= 256 ? 3 : 2;
+};
+
+// The join of `np` partials of `rows` rows (o [rows][HD], then m [rows], l [rows] each `stride`
+// floats apart): every thread takes part; result rows go to out/lse or to another partial.
+template <int HD>
+__device__ __forceinline__ void join_partials(const PagedAttn &a, const float *parts, long long stride, int np, int rows,
+                                              float *to, const SeqSpan &s, int kvh, int row0, float bits, float *fsh) {
+  // fsh: [np][rows] factors, then [rows] 1 / l.
+  const int t = threadIdx.x, nt = blockDim.x;
+  for (int r = t; r < rows; r += nt) {
+    float M = -INFINITY;
+    for (int i = 0; i < np; i++) M = fmaxf(M, __ldcg(parts + i * stride + rows * HD + r));
+    float l = 0.0f;
+    for (int i = 0; i < np; i++) {
+      const float m = __ldcg(parts + i * stride + rows * HD + r);
+      fsh[i * rows + r] = M == -INFINITY ? 0.0f : ex2(m - M);
+      l += rescale(__ldcg(parts + i * stride + rows * HD + rows + r), M == -INFINITY ? 0.0f : m - M);
+    }
+    fsh[np * rows + r] = l;
+    const int rr = row0 + r, i = rr / a.group;
+    if (to) {
+      to[rows * HD + r] = M;
+      to[rows * HD + rows + r] = l;
+    } else if (a.lse && i < s.n) {
+      a.lse[(long long)(s.row + i) * a.heads + kvh * a.group + rr % a.group] =
+          M == -INFINITY ? -INFINITY : (M - bits + log2f(l)) * kLn2;
+    }
+  }
+  __syncthreads();
+  for (int e = t; e < rows * (HD / 4); e += nt) {
+    const int r = e / (HD / 4), d = e % (HD / 4) * 4, rr = row0 + r, i = rr / a.group;
+    if (!to && i >= s.n) continue;
+    float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+    for (int k = 0; k < np; k++) {
+      const float f = fsh[k * rows + r];
+      const float4 v = __ldcg(reinterpret_cast<const float4 *>(parts + k * stride + r * HD + d));
+      o.x = fmaf(f, v.x, o.x);
+      o.y = fmaf(f, v.y, o.y);
+      o.z = fmaf(f, v.z, o.z);
+      o.w = fmaf(f, v.w, o.w);
+    }
+    if (to) {
+      *reinterpret_cast<float4 *>(to + r * HD + d) = o;
       continue;
     }
-    const long long row = ((long long)page * p.kv_heads + kvh) * p.page_size + t % p.page_size;
-    float dot = 0.0f;
-    for (int j = 0; j < hd / 32; j++) dot = fmaf(q[j], paged_code(p, p.k, row, j * 32 + lane), dot);
-    dot = warp_sum_bfly(dot) * a.scale * (p.ks ? p.ks[row] : 1.0f);
-    const float vs = p.vs ? p.vs[row] : 1.0f;
-    const float mn = fmaxf(m, dot + logf(fmaxf(vs, 0x1p-100f))), r = expf(m - mn), w = expf(dot - mn);
-    l = l * r + w;
-    for (int j = 0; j < hd / 32; j++) o[j] = fmaf(w * vs, paged_code(p, p.v, row, j * 32 + lane), o[j] * r);
-    m = mn;
+    const float l = fsh[np * rows + r], inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    const long long at = (long long)(s.row + i) * a.o_stride + (long long)(kvh * a.group + rr % a.group) * HD + d;
+    if (a.type == G4_F32) {
+      *reinterpret_cast<float4 *>((float *)a.out + at) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    } else {
+      const __nv_bfloat162 u = __floats2bfloat162_rn(o.x * inv, o.y * inv), v = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+      *reinterpret_cast<uint2 *>((__nv_bfloat16 *)a.out + at) =
+          make_uint2(*reinterpret_cast<const uint32_t *>(&u), *reinterpret_cast<const uint32_t *>(&v));
+    }
   }
-  const long long oo = (long long)(s.row + i) * a.o_stride + (long long)h * hd;
-  for (int j = 0; j < hd / 32; j++) {
-    const float v = l > 0.0f ? o[j] / l : 0.0f;
-    const int d = j * 32 + lane;
-    if (a.type == G4_F32)
-      ((float *)a.out)[oo + d] = v;
-    else
-      ((__nv_bfloat16 *)a.out)[oo + d] = __float2bfloat16_rn(v);
-  }
-  if (lane == 0 && a.lse) a.lse[(long long)(s.row + i) * a.heads + h] = m + logf(l);
 }
 
-size_t paged_attention_partials(const PagedAttn &) { return 0; }
+// Block (row group x KV head, split, sequence): 8 RT rows; RT warps share each tile of positions,
+// one row tile of 8 each, and 4 / RT tiles are worked on side by side.
+template <int FMT, int HD, int NP, int RT>
+__global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP>::OCC) k_paged_decode(const PagedAttn a) {
+  using S = DecShape<FMT, HD, NP>;
+  constexpr bool HALF = S::HALF;
+  constexpr int TG = kDecWarps / RT, ROWS = 8 * RT;
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31, g = lane >> 2, c = lane & 3;
+  const int rt = warp % RT, tg = warp / RT;
+  const int split = blockIdx.y, rg = blockIdx.x % a.row_groups, kvh = blockIdx.x / a.row_groups, b = blockIdx.z;
+  const SeqSpan s = seq_span(a, b);
+  const int R = s.n * a.group, row0 = rg * ROWS;
+  if (row0 >= R) return;
+  int lo, hi, tmp;
+  row_range(a, s.pos + row0 / a.group, s.kv, lo, tmp);
+  row_range(a, s.pos + (min(row0 + ROWS, R) - 1) / a.group, s.kv, tmp, hi);
+  const int first = lo >> 4, last = hi > lo ? (hi + 15) >> 4 : first;
+  const int ns = max(1, (last - first + a.split_tiles - 1) / a.split_tiles);
+  if (split >= ns) return;
+  const int tile0 = first + split * a.split_tiles, tile1 = min(last, tile0 + a.split_tiles);
 
-cudaError_t launch_paged_attention(const PagedAttn &a, cudaStream_t st) {
-  const dim3 grid((unsigned)(((long long)a.max_q * a.heads + 3) / 4), (unsigned)a.batch);
-  return launch_k(k_paged_attention, grid, dim3(128), 0, st, false, a);
+  extern __shared__ __align__(16) uint8_t dsm[];
+  uint2 *qs = reinterpret_cast<uint2 *>(dsm);   // [RT][NP][KSTEPS][32]
+  __shared__ float q_scale[ROWS];
+  __shared__ int row_lo[ROWS], row_hi[ROWS];
+
+  // ---- Q into fragment order: for K step k of row tile r lane (g, c) holds four consecutive
+  // dimensions of row g. One warp a row.
+  for (int r = warp; r < ROWS; r += kDecWarps) {
+    const int rr = row0 + r, i = rr / a.group;
+    const bool on = rr < R;
+    float x[HD / 32];
+    // Lane l takes dimensions 4 l' .. + 3 of each 128.
+    float top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < (HD + 127) / 128; j++) {
+      const int d = 128 * j + 4 * lane;
+      float4 v = make_float4(0, 0, 0, 0);
+      if (on && d < HD) {
+        const long long at = (long long)(s.row + i) * a.q_stride + (long long)(kvh * a.group + rr % a.group) * HD + d;
+        if (a.type == G4_F32) {
+          v = *reinterpret_cast<const float4 *>((const float *)a.q + at);
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2 *>((const __nv_bfloat16 *)a.q + at);
+          v = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                          __uint_as_float(u.y & 0xffff0000u));
+        }
+      }
+      if constexpr (HD >= 128) {
+        x[4 * j] = v.x; x[4 * j + 1] = v.y; x[4 * j + 2] = v.z; x[4 * j + 3] = v.w;
+      }
+      top = fmaxf(fmaxf(fmaxf(top, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
+      if constexpr (HD < 128) {
+        x[0] = v.x; x[1] = v.y;   // lanes 0..15 hold four; the rest of them below
+      }
+      if constexpr (HD < 128) {
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+        int e = (int)((__float_as_uint(top) >> 23) & 0xff) - 127;
+        if (!HALF || e < -110 || e > 127) e = HALF && e < -110 ? -110 : 0;
+        const float f = HALF ? __uint_as_float((uint32_t)(127 + 8 - e) << 23) : 1.0f;
+        uint32_t p01[NP], p23[NP];
+        split2<HALF, NP>(v.x * f, v.y * f, p01);
+        split2<HALF, NP>(v.z * f, v.w * f, p23);
+        if (d < HD) {
+          // 8 bit: d = 64 m + 16 c + 4 j, step 4 m + j; 16 bit: d = 32 m + 8 c + 4 j, step 2 m + j.
+          const int step = HALF ? (d >> 6) * 4 + ((d >> 2) & 3) : (d >> 5) * 2 + ((d >> 2) & 1);
+          const int cc = HALF ? (d >> 4) & 3 : (d >> 3) & 3;
+#pragma unroll
+          for (int k = 0; k < NP; k++)
+            qs[(((r >> 3) * NP + k) * S::KSTEPS + step) * 32 + (r & 7) * 4 + cc] = make_uint2(p01[k], p23[k]);
+        }
+        if (lane == 0) q_scale[r] = a.scale * kLog2e * (HALF ? __uint_as_float((uint32_t)(127 - 8 + e) << 23) : 1.0f);
+      }
+    }
+    if constexpr (HD >= 128) {
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+      int e = (int)((__float_as_uint(top) >> 23) & 0xff) - 127;
+      if (!HALF || e < -110 || e > 127) e = HALF && e < -110 ? -110 : 0;
+      const float f = HALF ? __uint_as_float((uint32_t)(127 + 8 - e) << 23) : 1.0f;
+#pragma unroll
+      for (int j = 0; j < HD / 128; j++) {
+        const int d = 128 * j + 4 * lane;
+        uint32_t p01[NP], p23[NP];
+        split2<HALF, NP>(x[4 * j] * f, x[4 * j + 1] * f, p01);
+        split2<HALF, NP>(x[4 * j + 2] * f, x[4 * j + 3] * f, p23);
+        const int step = HALF ? (d >> 6) * 4 + ((d >> 2) & 3) : (d >> 5) * 2 + ((d >> 2) & 1);
+        const int cc = HALF ? (d >> 4) & 3 : (d >> 3) & 3;
+#pragma unroll
+        for (int k = 0; k < NP; k++)
+          qs[(((r >> 3) * NP + k) * S::KSTEPS + step) * 32 + (r & 7) * 4 + cc] = make_uint2(p01[k], p23[k]);
+      }
+      if (lane == 0) q_scale[r] = a.scale * kLog2e * (HALF ? __uint_as_float((uint32_t)(127 - 8 + e) << 23) : 1.0f);
+    }
+    if (lane == 0) {
+      int x0 = 0, x1 = 0;
+      if (on) row_range(a, s.pos + i, s.kv, x0, x1);
+      row_lo[r] = x0;
+      row_hi[r] = x1;
+    }
+  }
+  __syncthreads();
+
+  const float qf0 = q_scale[rt * 8 + 2 * c], qf1 = q_scale[rt * 8 + 2 * c + 1];
+  const int lo0 = row_lo[rt * 8 + 2 * c], hi0 = row_hi[rt * 8 + 2 * c];
+  const int lo1 = row_lo[rt * 8 + 2 * c + 1], hi1 = row_hi[rt * 8 + 2 * c + 1];
+  // Positions that every row of this warp sees need no mask.
+  const int rv = min(8, R - row0 - rt * 8);   // rows of this warp's tile that exist
+  int all_lo = 0, all_hi = 0;
+  if (rv > 0) {
+    all_lo = row_lo[rt * 8 + rv - 1];
+    all_hi = row_hi[rt * 8];
+  }
+  const uint2 *qw = qs + (size_t)rt * NP * S::KSTEPS * 32 + lane;
+
+  float o[HD / 16][4];
+#pragma unroll
+  for (int i = 0; i < HD / 16; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+
+  // ---- this warp's tiles: tile0 + tg + TG n. Lane i holds the page of the i-th of 32 ahead.
+  const Pool &p = a.pool;
+  const int mine = tile1 - tile0 - tg > 0 ? (tile1 - tile0 - tg + TG - 1) / TG : 0;
+  const int per_page = p.page_size >> 4;
+  const int32_t *table = a.table + (long long)b * a.table_stride;
+  int pages = -1, pages_at = 0;
+  auto fetch_pages = [&](int n) {
+    const int k = n + lane;
+    pages = k < mine ? table[(tile0 + tg + TG * k) / per_page] : -1;
+    if (k < mine && (pages < 0 || pages >= p.n_pages)) {
+      paged_raise(a.err, G4_PAGED_BAD_PAGE);
+      pages = -1;
+    }
+    pages_at = n;
+  };
+  // Position row (in rows of the pool) of the n-th tile's first position; -1 where its page is none.
+  auto tile_row = [&](int n) -> long long {
+    const int page = __shfl_sync(0xffffffffu, pages, (n - pages_at) & 31);
+    const int tile = tile0 + tg + TG * n;
+    return page < 0 ? -1 : ((long long)page * p.kv_heads + kvh) * p.page_size + (tile % per_page) * 16;
+  };
+
+  uint4 buf[S::NB][4];
+  // Chunk q of the tile whose first row is `row`: K chunks first, then V.
+  auto load_chunk = [&](uint4 (&d)[4], int q, long long row) {
+    if (row < 0) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) d[i] = make_uint4(0, 0, 0, 0);
+      return;
+    }
+    auto ld16 = [&](const uint8_t *at) { return RT == 1 ? ldg_stream(at) : __ldg(reinterpret_cast<const uint4 *>(at)); };
+    if (q < S::HC) {
+      const uint8_t *k = p.k + row * S::ROW + g * S::ROW + c * 16 + q * 128;
+      d[0] = ld16(k);
+      d[1] = ld16(k + 8 * S::ROW);
+      if (!S::NARROW) {
+        d[2] = ld16(k + 64);
+        d[3] = ld16(k + 64 + 8 * S::ROW);
+      }
+    } else {
+      const uint8_t *v = p.v + row * S::ROW + 2 * c * S::ROW + (S::NARROW ? g * 8 : g * 16 + (q - S::HC) * 128);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const uint8_t *at = v + ((i & 1) + (i >> 1) * 8) * S::ROW;
+        if (S::NARROW) {
+          const uint2 w = __ldg(reinterpret_cast<const uint2 *>(at));
+          d[i] = make_uint4(w.x, w.y, 0, 0);
+        } else {
+          d[i] = ld16(at);
+        }
+      }
+    }
+  };
+  // Scales of positions g and g + 8 of the tile.
+  float ks0 = 1.0f, ks1 = 1.0f, vs0 = 1.0f, vs1 = 1.0f;
+  auto load_scales = [&](long long row) {
+    if (HALF && row >= 0) {
+      ks0 = __ldg(p.ks + row + g);
+      ks1 = __ldg(p.ks + row + g + 8);
+      vs0 = __ldg(p.vs + row + g);
+      vs1 = __ldg(p.vs + row + g + 8);
+    }
+  };
+
+  // Rows of the tiles the ring reaches into: [0] the one at hand.
+  long long rows_[S::TILES + 2];
+  if (mine > 0) fetch_pages(0);
+#pragma unroll
+  for (int i = 0; i < S::TILES + 2; i++) rows_[i] = i < mine ? tile_row(i) : -1;
+  load_scales(rows_[0]);
+#pragma unroll
+  for (int q = 0; q < S::NB - 1; q++) load_chunk(buf[q], q % S::C, rows_[q / S::C]);
+
+  for (int n0 = 0; n0 < mine; n0 += S::TILES) {
+#pragma unroll
+    for (int u = 0; u < S::TILES; u++) {
+      const int n = n0 + u;
+      const bool on = n < mine && rows_[u] >= 0;   // the same for the whole warp
+      const int pos0 = (tile0 + tg + TG * n) * 16;
+      float sa[4] = {0, 0, 0, 0}, sb[4] = {0, 0, 0, 0};
+      uint32_t pw[2][NP];
+      uint32_t dead = 0;
+#pragma unroll
+      for (int q = 0; q < S::C; q++) {
+        const int at = u * S::C + q;
+        {
+          const int ahead = at + S::NB - 1;
+          load_chunk(buf[ahead % S::NB], ahead % S::C, rows_[ahead / S::C]);
+        }
+        const uint4 (&w)[4] = buf[at % S::NB];
+        if (q < S::HC) {
+#pragma unroll
+          for (int h = 0; h < (S::NARROW ? 1 : 2); h++) {
+            const uint32_t r0[4] = {w[2 * h].x, w[2 * h].y, w[2 * h].z, w[2 * h].w};
+            const uint32_t r1[4] = {w[2 * h + 1].x, w[2 * h + 1].y, w[2 * h + 1].z, w[2 * h + 1].w};
+            constexpr int ST = HALF ? 4 : 2;
+#pragma unroll
+            for (int j = 0; j < ST; j++) {
+              uint32_t a0, a1, a2, a3;
+              if constexpr (HALF) {
+                codes4<FMT>(r0[j], a0, a2);
+                codes4<FMT>(r1[j], a1, a3);
+              } else {
+                a0 = r0[2 * j];
+                a2 = r0[2 * j + 1];
+                a1 = r1[2 * j];
+                a3 = r1[2 * j + 1];
+              }
+              const int step = (q * 2 + h) * ST + j;
+#pragma unroll
+              for (int k = 0; k < NP; k++) {
+                const uint2 bq = qw[(k * S::KSTEPS + step) * 32];
+                if (step & 1)
+                  mma16816<HALF>(sb, a0, a1, a2, a3, bq.x, bq.y);
+                else
+                  mma16816<HALF>(sa, a0, a1, a2, a3, bq.x, bq.y);
+              }
+            }
+          }
+        }
+        if (q == S::HC - 1) {
+          // ---- softmax of the tile: sa[0], sa[1] are position g of rows 2c, 2c + 1; sa[2], sa[3] g + 8.
+          float s0 = (sa[0] + sb[0]) * (ks0 * qf0), s1 = (sa[1] + sb[1]) * (ks0 * qf1);
+          float s2 = (sa[2] + sb[2]) * (ks1 * qf0), s3 = (sa[3] + sb[3]) * (ks1 * qf1);
+          float w0 = vs0, w1 = vs1;
+          bool see0 = on, see1 = on, see2 = on, see3 = on;
+          const bool whole = on && pos0 >= all_lo && pos0 + 16 <= all_hi;
+          if (!whole && on) {
+            const int t0 = pos0 + g, t1 = t0 + 8;
+            see0 = t0 >= lo0 && t0 < hi0;
+            see1 = t0 >= lo1 && t0 < hi1;
+            see2 = t1 >= lo0 && t1 < hi0;
+            see3 = t1 >= lo1 && t1 < hi1;
+            // Positions whose V must not enter the product: those outside every row's range, and
+            // in bf16 pages those that hold an infinity or a NaN (0 times it is NaN for a row
+            // that does not see it); the rows that do see one get a NaN weight.
+            const unsigned live0 = __ballot_sync(0xffffffffu, see0 || see1), live1 = __ballot_sync(0xffffffffu, see2 || see3);
+            uint32_t live = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              if ((live0 >> (4 * i)) & 0xf) live |= 1u << i;
+              if ((live1 >> (4 * i)) & 0xf) live |= 1u << (i + 8);
+            }
+            dead = ~live & 0xffffu;
+            if constexpr (!HALF) {
+              uint32_t bad = 0;
+              for (int i = 0; i < 16; i++) {
+                const uint8_t *v = p.v + (rows_[u] + i) * S::ROW;
+                bool x = false;
+                for (int d = lane; d < HD / 2; d += 32) {
+                  const uint32_t z = *reinterpret_cast<const uint32_t *>(v + 4 * d);
+                  x |= (z & 0x7f80u) == 0x7f80u || (z & 0x7f800000u) == 0x7f800000u;
+                }
+                if (__any_sync(0xffffffffu, x)) bad |= 1u << i;
+              }
+              dead |= bad;
+              if ((bad >> g) & 1) w0 = __int_as_float(0x7fffffff);
+              if ((bad >> (g + 8)) & 1) w1 = __int_as_float(0x7fffffff);
+            }
+          }
+          const float g0 = HALF ? __log2f(fmaxf(w0, 0x1p-100f)) : 0.0f, g1 = HALF ? __log2f(fmaxf(w1, 0x1p-100f)) : 0.0f;
+          s0 = see0 ? s0 : -INFINITY;
+          s1 = see1 ? s1 : -INFINITY;
+          s2 = see2 ? s2 : -INFINITY;
+          s3 = see3 ? s3 : -INFINITY;
+          float n0_ = fmaxf(s0 + g0, s2 + g1), n1_ = fmaxf(s1 + g0, s3 + g1);
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) {
+            n0_ = fmaxf(n0_, __shfl_xor_sync(0xffffffffu, n0_, x));
+            n1_ = fmaxf(n1_, __shfl_xor_sync(0xffffffffu, n1_, x));
+          }
+          n0_ = fmaxf(n0_, m0);
+          n1_ = fmaxf(n1_, m1);
+          if (__any_sync(0xffffffffu, n0_ > m0 || n1_ > m1)) {
+            const float f0 = n0_ > m0 ? ex2(m0 - n0_) : 1.0f, f1 = n1_ > m1 ? ex2(m1 - n1_) : 1.0f;
+            l0 = n0_ > m0 ? rescale(l0, m0 - n0_) : l0;
+            l1 = n1_ > m1 ? rescale(l1, m1 - n1_) : l1;
+#pragma unroll
+            for (int i = 0; i < HD / 16; i++) {
+              o[i][0] *= f0;
+              o[i][1] *= f1;
+              o[i][2] *= f0;
+              o[i][3] *= f1;
+            }
+            m0 = n0_;
+            m1 = n1_;
+          }
+          const float bits = HALF ? kWeightBits : 0.0f;
+          const float r0 = m0 == -INFINITY ? 0.0f : m0 - bits, r1 = m1 == -INFINITY ? 0.0f : m1 - bits;
+          const float p0 = ex2(s0 - r0), p1 = ex2(s1 - r1), p2 = ex2(s2 - r0), p3 = ex2(s3 - r1);
+          l0 += p0 + p2;
+          l1 += p1 + p3;
+          uint32_t x[NP], y[NP];
+          split2<HALF, NP>(see0 ? p0 * w0 : 0.0f, see1 ? p1 * w0 : 0.0f, x);
+          split2<HALF, NP>(see2 ? p2 * w1 : 0.0f, see3 ? p3 * w1 : 0.0f, y);
+#pragma unroll
+          for (int k = 0; k < NP; k++) {
+            pw[0][k] = transpose8x8(x[k]);
+            pw[1][k] = transpose8x8(y[k]);
+          }
+          load_scales(u + 1 < S::TILES ? rows_[u + 1] : rows_[S::TILES]);
+        }
+        if (q >= S::HC) {
+          uint4 v[4] = {w[0], w[1], w[2], w[3]};
+          if (dead) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              if ((dead >> (2 * c + (i & 1) + (i >> 1) * 8)) & 1) v[i] = make_uint4(0, 0, 0, 0);
+          }
+          const uint32_t vw[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
+                                     {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
+          constexpr int WORDS = S::NARROW ? 2 : 4;
+          const int ob = (q - S::HC) * (HALF ? 8 : 4);
+#pragma unroll
+          for (int j = 0; j < WORDS; j++) {
+            if constexpr (HALF) {
+              // Four dimensions of the pairs (2c, 2c + 1) and (2c + 8, 2c + 9).
+              uint32_t e[2][4];
+#pragma unroll
+              for (int h = 0; h < 2; h++) {
+                const uint32_t t0 = __byte_perm(vw[2 * h][j], vw[2 * h + 1][j], 0x5140);
+                const uint32_t t1 = __byte_perm(vw[2 * h][j], vw[2 * h + 1][j], 0x7362);
+                codes4<FMT>(t0, e[h][0], e[h][1]);
+                codes4<FMT>(t1, e[h][2], e[h][3]);
+              }
+#pragma unroll
+              for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int k = 0; k < NP; k++)
+                  mma16816<HALF>(o[ob + 2 * j + i], e[0][2 * i], e[0][2 * i + 1], e[1][2 * i], e[1][2 * i + 1], pw[0][k], pw[1][k]);
+            } else {
+              const uint32_t a0 = __byte_perm(vw[0][j], vw[1][j], 0x5410), a1 = __byte_perm(vw[0][j], vw[1][j], 0x7632);
+              const uint32_t a2 = __byte_perm(vw[2][j], vw[3][j], 0x5410), a3 = __byte_perm(vw[2][j], vw[3][j], 0x7632);
+#pragma unroll
+              for (int k = 0; k < NP; k++) mma16816<HALF>(o[ob + j], a0, a1, a2, a3, pw[0][k], pw[1][k]);
+            }
+          }
+        }
+      }
+    }
+    // The next pass's tiles.
+    if (n0 + S::TILES < mine) {
+      const int base = n0 + S::TILES;
+#pragma unroll
+      for (int i = 0; i < 2; i++) rows_[i] = rows_[S::TILES + i];
+      if (base + S::TILES + 1 - pages_at >= 32) fetch_pages(base);
+#pragma unroll
+      for (int i = 2; i < S::TILES + 2; i++) rows_[i] = base + i < mine ? tile_row(base + i) : -1;
+    }
+  }
+
+  // ---- join the token groups through shared memory (over Q), then write out or leave a partial.
+#pragma unroll
+  for (int x = 4; x < 32; x <<= 1) {
+    l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+  }
+  __syncthreads();
+  // Partials [TG]: o [ROWS][HD], m [ROWS], l [ROWS].
+  constexpr int PART = ROWS * (HD + 2);
+  float *sm = reinterpret_cast<float *>(dsm) + tg * PART;
+#pragma unroll
+  for (int q = 0; q < HD / 16; q++) {
+    // Accumulator q: the chunk's dimensions 16 g + 2 j (8 bit; 8 g + 2 j narrow or at 16 bits) and the next.
+    constexpr int PER = S::NARROW ? 4 : (HALF ? 8 : 4);
+    const int chunk = q / PER, j = q % PER;
+    const int d = chunk * (HALF && !S::NARROW ? 128 : 64) + g * (HALF && !S::NARROW ? 16 : 8) + 2 * j;
+    *reinterpret_cast<float2 *>(sm + (rt * 8 + 2 * c) * HD + d) = make_float2(o[q][0], o[q][2]);
+    *reinterpret_cast<float2 *>(sm + (rt * 8 + 2 * c + 1) * HD + d) = make_float2(o[q][1], o[q][3]);
+  }
+  if (g == 0) {
+    sm[ROWS * HD + rt * 8 + 2 * c] = m0;
+    sm[ROWS * HD + rt * 8 + 2 * c + 1] = m1;
+    sm[ROWS * HD + ROWS + rt * 8 + 2 * c] = l0;
+    sm[ROWS * HD + ROWS + rt * 8 + 2 * c + 1] = l1;
+  }
+  __syncthreads();
+  __shared__ float fsh[(kJoin + 1) * ROWS];
+  __shared__ bool is_last;
+  const float bits = HALF ? kWeightBits : 0.0f;
+  const long long slot0 = (((long long)b * p.kv_heads + kvh) * a.row_groups + rg) * a.splits;
+  float *mine_part = ns > 1 ? a.part + (slot0 + split) * PART : nullptr;
+  {
+    // The same join as between blocks, its partials in shared memory.
+    const float *sp = reinterpret_cast<const float *>(dsm);
+    for (int r = t; r < ROWS; r += kDecWarps * 32) {
+      float M = -INFINITY, l = 0.0f;
+      for (int i = 0; i < TG; i++) M = fmaxf(M, sp[i * PART + ROWS * HD + r]);
+      for (int i = 0; i < TG; i++) {
+        const float m = sp[i * PART + ROWS * HD + r];
+        fsh[i * ROWS + r] = M == -INFINITY ? 0.0f : ex2(m - M);
+        l += rescale(sp[i * PART + ROWS * HD + ROWS + r], M == -INFINITY ? 0.0f : m - M);
+      }
+      fsh[TG * ROWS + r] = l;
+      const int rr = row0 + r, i = rr / a.group;
+      if (mine_part) {
+        mine_part[ROWS * HD + r] = M;
+        mine_part[ROWS * HD + ROWS + r] = l;
+      } else if (a.lse && rr < R) {
+        a.lse[(long long)(s.row + i) * a.heads + kvh * a.group + rr % a.group] =
+            M == -INFINITY ? -INFINITY : (M - bits + log2f(l)) * kLn2;
+      }
+    }
+    __syncthreads();
+    for (int e = t; e < ROWS * (HD / 4); e += kDecWarps * 32) {
+      const int r = e / (HD / 4), d = e % (HD / 4) * 4, rr = row0 + r, i = rr / a.group;
+      float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll
+      for (int k = 0; k < TG; k++) {
+        const float f = fsh[k * ROWS + r];
+        const float4 z = *reinterpret_cast<const float4 *>(sp + k * PART + r * HD + d);
+        v.x = fmaf(f, z.x, v.x);
+        v.y = fmaf(f, z.y, v.y);
+        v.z = fmaf(f, z.z, v.z);
+        v.w = fmaf(f, z.w, v.w);
+      }
+      if (mine_part) {
+        *reinterpret_cast<float4 *>(mine_part + r * HD + d) = v;
+        continue;
+      }
+      if (rr >= R) continue;
+      const float l = fsh[TG * ROWS + r], inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+      const long long at = (long long)(s.row + i) * a.o_stride + (long long)(kvh * a.group + rr % a.group) * HD + d;
+      if (a.type == G4_F32) {
+        *reinterpret_cast<float4 *>((float *)a.out + at) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+      } else {
+        *reinterpret_cast<uint2 *>((__nv_bfloat16 *)a.out + at) = make_uint2(
+            [&] { const __nv_bfloat162 h = __floats2bfloat162_rn(v.x * inv, v.y * inv); return *reinterpret_cast<const uint32_t *>(&h); }(),
+            [&] { const __nv_bfloat162 h = __floats2bfloat162_rn(v.z * inv, v.w * inv); return *reinterpret_cast<const uint32_t *>(&h); }());
+      }
+    }
+  }
+  if (ns == 1) return;
+
+  // ---- the last of each group of kJoin splits joins it; the last group joins the groups.
+  const int groups = (ns + kJoin - 1) / kJoin, grp = split / kJoin;
+  const int in_group = min(kJoin, ns - grp * kJoin);
+  const int max_groups = (a.splits + kJoin - 1) / kJoin;
+  uint32_t *cnt = a.count + (slot0 / a.splits) * (max_groups + 1);
+  __threadfence();
+  __syncthreads();
+  if (t == 0) {
+    is_last = atomicAdd(cnt + 1 + grp, 1u) == (unsigned)in_group - 1;
+    if (is_last) cnt[1 + grp] = 0;
+  }
+  __syncthreads();
+  if (!is_last) return;
+  __threadfence();
+  float *base = a.part + (slot0 + (long long)grp * kJoin) * PART;
+  // A group's result replaces its first partial: each thread reads an element of all before it
+  // writes it, and the rows' statistics go through fsh.
+  join_partials<HD>(a, base, PART, in_group, ROWS, groups > 1 ? base : nullptr, s, kvh, row0, bits, fsh);
+  if (groups == 1) return;
+  __threadfence();
+  __syncthreads();
+  if (t == 0) {
+    is_last = atomicAdd(cnt, 1u) == (unsigned)groups - 1;
+    if (is_last) cnt[0] = 0;
+  }
+  __syncthreads();
+  if (!is_last) return;
+  __threadfence();
+  join_partials<HD>(a, a.part + slot0 * PART, (long long)kJoin * PART, groups, ROWS, nullptr, s, kvh, row0, bits, fsh);
+}
+
+// ------------------------------------------------------------------------------ launch
+// Row tiles per block: 1 for a group's 8 rows, up to 4 (each reads the positions again, from L1).
+static int decode_rt(const PagedAttn &a) {
+  const long long R = (long long)a.max_q * a.group;
+  return R <= 8 ? 1 : (R <= 16 ? 2 : 4);
+}
+
+// Fills in the split: enough blocks for two rounds of the SMs, no split below one tile a warp, at most
+// kJoin^2 of them.
+static void plan_decode(PagedAttn &a) {
+  const int rt = decode_rt(a), rows = 8 * rt, tg = kDecWarps / rt;
+  a.row_groups = (int)(((long long)a.max_q * a.group + rows - 1) / rows);
+  // Positions a row group can see: its queries' windows, from a tile boundary.
+  long long span = a.max_kv;
+  if (a.window > 0) {
+    const long long w = (long long)a.window + (rows + a.group - 1) / a.group + 16;
+    if (w < span) span = w;
+  }
+  const int tiles = (int)((span + 15) / 16) > 0 ? (int)((span + 15) / 16) : 1;
+  const long long base = (long long)a.batch * a.pool.kv_heads * a.row_groups;
+  const int occ = a.pool.hd <= 256 ? 3 : 2;
+  long long want = (2ll * 148 * occ + base - 1) / base;
+  const long long most = (tiles + tg - 1) / tg;
+  if (want > most) want = most;
+  if (want > kJoin * kJoin) want = kJoin * kJoin;
+  if (base * (want / kJoin + 2) > kPagedCounters) want = 1;
+  int per = (int)((tiles + want - 1) / want);
+  per = (per + tg - 1) / tg * tg;
+  a.split_tiles = per;
+  a.splits = (tiles + per - 1) / per;
+}
+
+size_t paged_attention_partials(const PagedAttn &args) {
+  PagedAttn a = args;
+  if (a.max_q < 1 || a.batch < 1) return 0;
+  plan_decode(a);
+  if (a.splits == 1) return 0;
+  return (size_t)a.batch * a.pool.kv_heads * a.row_groups * a.splits * (8 * decode_rt(a)) * (a.pool.hd + 2) * sizeof(float);
+}
+
+template <int FMT, int HD, int NP, int RT>
+static cudaError_t launch_decode_rt(const PagedAttn &a, cudaStream_t st) {
+  using S = DecShape<FMT, HD, NP>;
+  constexpr int QB = RT * NP * S::KSTEPS * 32 * 8, OB = kDecWarps / RT * 8 * RT * (HD + 2) * 4;
+  constexpr int SMEM = QB > OB ? QB : OB;
+  static DeviceOnce once;
+  cudaError_t e = cudaSuccess;
+  once([&] { e = cudaFuncSetAttribute(k_paged_decode<FMT, HD, NP, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); });
+  if (e != cudaSuccess) return e;
+  const dim3 grid(a.row_groups * a.pool.kv_heads, a.splits, a.batch);
+  return launch_k(k_paged_decode<FMT, HD, NP, RT>, grid, dim3(kDecWarps * 32), SMEM, st, false, a);
+}
+template <int FMT, int HD, int NP>
+static cudaError_t launch_decode_np(const PagedAttn &a, cudaStream_t st) {
+  switch (decode_rt(a)) {
+    case 1: return launch_decode_rt<FMT, HD, NP, 1>(a, st);
+    case 2: return launch_decode_rt<FMT, HD, NP, 2>(a, st);
+    default: return launch_decode_rt<FMT, HD, NP, 4>(a, st);
+  }
+}
+template <int FMT, int HD>
+static cudaError_t launch_decode_hd(const PagedAttn &a, cudaStream_t st) {
+  if (a.type == G4_BF16) return launch_decode_np<FMT, HD, 1>(a, st);
+  return launch_decode_np<FMT, HD, FMT == G4_PAGE_BF16 ? 3 : 2>(a, st);
+}
+template <int FMT>
+static cudaError_t launch_decode(const PagedAttn &a, cudaStream_t st) {
+  switch (a.pool.hd) {
+    case 64: return launch_decode_hd<FMT, 64>(a, st);
+    case 128: return launch_decode_hd<FMT, 128>(a, st);
+    case 256: return launch_decode_hd<FMT, 256>(a, st);
+    default: return launch_decode_hd<FMT, 512>(a, st);
+  }
+}
+
+cudaError_t launch_paged_attention(const PagedAttn &args, cudaStream_t st) {
+  PagedAttn a = args;
+  plan_decode(a);
+  switch (a.pool.fmt) {
+    case G4_PAGE_BF16: return launch_decode<G4_PAGE_BF16>(a, st);
+    case G4_PAGE_INT8: return launch_decode<G4_PAGE_INT8>(a, st);
+    default: return launch_decode<G4_PAGE_E4M3>(a, st);
+  }
 }
 
 }  // namespace g4

@@ -4,8 +4,9 @@ against their definitions in 64 bits, at the sizes and masks where they can go w
 Tolerances. Stored codes and what is read back are exact: the same f32 operations in the same
 order. Attention, with A = max_t scale * sum_d |q_d k_td| of the row and B_d = sum_t p_t |v_td|:
 scores accumulate exact products in f32, so a score is off by at most 2^-21 A and its weight by as
-much relatively; bf16 rows add the rounding of the weights (2^-9 each) and of the result (2^-9);
-f32 rows carry q and the weights in parts of at least 22 bits together. Weights are held relative to
+much relatively; bf16 rows add the rounding of the result (2^-8, bf16's unit roundoff: 1 + 2^-8
+rounds to 1) and of the weights (2^-8 each in bf16 pages, whose products are bf16, 2^-11 in 8-bit
+pages, whose products are f16); f32 rows carry q and the weights in parts of at least 22 bits together. Weights are held relative to
 the largest of their row in a type with a smallest step: F bounds what n of them below that step
 add, 2^-126 of the largest for bf16 pages (f32's exponents) and 2^-38 for 8-bit pages (f16 parts
 scaled by 2^14), which shows only where the heavy positions' codes are zero; results below the
@@ -225,8 +226,8 @@ def reference(torch, pool, q, spans, table, window, scale):
     return out, lse, A, B, F
 
 
-def check(torch, got, glse, want, lse, A, B, F, bf16):
-    tol = (2.0 ** -21 * 2 * A + (2.0 ** -8 + 2.0 ** -11 if bf16 else 2.0 ** -19)) * B + F + 2.0 ** -126
+def check(torch, got, glse, want, lse, A, B, F, bf16, pages16=False):
+    tol = (2.0 ** -21 * 2 * A + (2.0 ** -8 + 2.0 ** -11 + (2.0 ** -8 if pages16 else 0) if bf16 else 2.0 ** -19)) * B + F + 2.0 ** -126
     off = (got.double() - want).abs()
     assert not got.isnan().any()
     bad = off > tol
@@ -281,7 +282,7 @@ def run_case(paged, torch, q_len, kv, heads, kv_heads, hd, page, fmt, dtype, win
     for a, b in ((0, gap), (rows - gap, rows)):   # rows of no sequence stay as they were
         assert (out[a:b] == 7).all() and (lse[a:b] == 7).all()
     sl = slice(gap, rows - gap)
-    check(torch, out[sl], lse[sl], want[sl], wl[sl], A[sl], B[sl], F[sl], dtype == "bf16")
+    check(torch, out[sl], lse[sl], want[sl], wl[sl], A[sl], B[sl], F[sl], dtype == "bf16", fmt == "bf16")
     return out
 
 

@@ -16,7 +16,8 @@ CSRC = PKG / "csrc"
 LIB_DIR = PKG / "lib"
 LIB = LIB_DIR / "libgemma4_cuda.so"
 SOURCES = ["g4_kernels.cu", "g4_gemv2.cu", "g4_gemm.cu", "g4_ple.cu", "g4_runtime.cu", "g4_noalloc.cu",
-           "g4_paged.cu", "g4_paged_attn.cu", "g4_drafts.cu"]
+           "g4_paged.cu", "g4_paged_attn.cu", "g4_paged_chunk.cu",
+           "g4_drafts.cu"]
 HEADERS = ["g4_device.cuh", "g4_kernels.cuh", "g4_gemv.cuh", "g4_paged.cuh"]
 
 NVCC_FLAGS = [

@@ -98,6 +98,8 @@ __device__ __forceinline__ void row_range(const PagedAttn &a, int p, int kv, int
 }
 
 cudaError_t launch_paged_attention(const PagedAttn &a, cudaStream_t st);
+// Chunks of bf16 rows (g4_paged_chunk.cu).
+cudaError_t launch_paged_chunk(const PagedAttn &a, cudaStream_t st);
 // Bytes of partials a call of this shape needs past the counters.
 size_t paged_attention_partials(const PagedAttn &a);
 

@@ -668,6 +668,9 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP>::OCC) k_
 }
 
 // ------------------------------------------------------------------------------ launch
+// More rows per KV head than a block here holds: the chunk kernel's 128-row tiles.
+static bool chunk_path(const PagedAttn &a) { return a.type == G4_BF16 && (long long)a.max_q * a.group > 32; }
+
 // Row tiles per block: 1 for a group's 8 rows, up to 4 (each reads the positions again, from L1).
 static int decode_rt(const PagedAttn &a) {
   const long long R = (long long)a.max_q * a.group;
@@ -701,7 +704,7 @@ static void plan_decode(PagedAttn &a) {
 
 size_t paged_attention_partials(const PagedAttn &args) {
   PagedAttn a = args;
-  if (a.max_q < 1 || a.batch < 1) return 0;
+  if (a.max_q < 1 || a.batch < 1 || chunk_path(a)) return 0;
   plan_decode(a);
   if (a.splits == 1) return 0;
   return (size_t)a.batch * a.pool.kv_heads * a.row_groups * a.splits * (8 * decode_rt(a)) * (a.pool.hd + 2) * sizeof(float);
@@ -744,6 +747,7 @@ static cudaError_t launch_decode(const PagedAttn &a, cudaStream_t st) {
 
 cudaError_t launch_paged_attention(const PagedAttn &args, cudaStream_t st) {
   PagedAttn a = args;
+  if (chunk_path(a)) return launch_paged_chunk(a, st);
   plan_decode(a);
   switch (a.pool.fmt) {
     case G4_PAGE_BF16: return launch_decode<G4_PAGE_BF16>(a, st);

@@ -11,12 +11,14 @@
 //    of its S as f16 (bf16 pages: bf16) and is the second product's A operand from there.
 //  - K and V pass through one ring of 16 KB slots, each [128 positions][64 dimensions] 16-bit in
 //    the 128-byte swizzle: K-major B operand of the first product, and the same bytes are the
-//    MN-major B operand of the second, so both are written alike. Eight producer warps gather the
-//    pages' rows: 8-bit codes through registers (six slots in flight), widened to f16; bf16 rows by
-//    asynchronous copies.
+//    MN-major B operand of the second, so both are written alike. Six producer warps gather the
+//    pages' rows, each a slot of its own: 8-bit codes through registers, the next slot's requested
+//    as this one's are widened to f16, bf16 rows by asynchronous copies. A scout warp reads the
+//    page table and the scales blocks ahead.
 //  - One thread issues the products in the order S(j), O(j - 1), so the softmax of block j runs
 //    under the products of its neighbours.
-//  - Softmax: one thread a row. The maximum is stale by up to a factor of 2^1.9 (weights stay
+//  - Softmax: two threads a row, 64 positions of a block each, held in registers from the scores to
+//    the weights. The maximum is stale by up to a factor of 2^1.9 (weights stay
 //    below f16's greatest number); only when a row outgrows it are its warp's O rows rescaled.
 // head_dim 512: O would fill tensor memory alone, so two blocks compute the scores each and take
 // half of V's dimensions (1.5 times the operations).
@@ -31,12 +33,25 @@ namespace g4 {
 
 namespace {
 
-constexpr int kProducers = 256, kSoftmax = 128;
-constexpr int kThreads = kSoftmax + kProducers + 32;
+// Warps by role: softmax, producers, the scout, the products.
+constexpr int kSoftWarps = 8, kProdWarps = 6;
+constexpr int kScout = kSoftWarps + kProdWarps, kMma = kScout + 1;
+constexpr int kThreads = 32 * (kMma + 1);
 constexpr int BN = 128;            // positions per block
 constexpr int SLOT = BN * 128;     // bytes of a slot
-constexpr int NSC = 4;             // buffers of a block's scales
+constexpr int NSC = 8;             // buffers of what the scout found out about a block
 constexpr float kL2e = 1.44269504088896341f, kLn2f = 0.693147180559945309f;
+
+// A block of positions as the scout leaves it: their scales (vs < 0: no page there), log2 of the V
+// scales, the byte offset of each 16 positions' rows in the pool (-1: none), the greatest log2, and
+// whether one bound serves all (every page there, scales within 2^8 of each other).
+struct BlockInfo {
+  float ks[BN], vs[BN], lv[BN];
+  long long at[BN / 16];
+  float lmax;
+  int even;
+  int pad[2];
+};
 
 template <int FMT, int HD>
 struct ChunkShape {
@@ -45,11 +60,15 @@ struct ChunkShape {
   static constexpr int OD = HD < 256 ? HD : 256;        // dimensions of O a block accumulates
   static constexpr int VC = OD / 64;                    // V slots of a block
   static constexpr int NS = HD == 512 ? 5 : 9;          // ring slots
-  static constexpr int AHEAD = HD == 512 ? 4 : 6;       // slots in flight ahead of the ring's writes
+  // Producer warps: warp w fills slots w, w + PW, ... A slot's rounds are told apart by one parity bit, so
+  // whoever waits for a round must know that the one before it has ended: PW <= NS gives that, as
+  // the warp's own last slot is then consumed no earlier than the slot it waits for was filled.
+  static constexpr int PW = HD == 512 ? 5 : kProdWarps;
+  static_assert(PW == NS || NS >= PW + 3, "see PW");
   static constexpr int Q_BYTES = KC * SLOT;
-  static constexpr int SC_OFF = Q_BYTES + NS * SLOT;    // [NSC][3][BN] floats: ks, vs, log2 vs
-  static constexpr int BAR_OFF = SC_OFF + NSC * 3 * BN * 4;
-  // full[NS], empty[NS], s_full[2], p_ready[2], pv_done, sc_full[NSC], sc_free[NSC], end
+  static constexpr int SC_OFF = Q_BYTES + NS * SLOT;
+  static constexpr int BAR_OFF = SC_OFF + NSC * (int)sizeof(BlockInfo);
+  // full[NS], empty[NS], s_full[2], p_ready[2], pv_done, info_full[NSC], info_free[NSC], end
   static constexpr int BARS = 2 * NS + 2 + 2 + 1 + 2 * NSC + 1;
   static constexpr int SMEM = BAR_OFF + BARS * 8 + 64 + 1024;
 };
@@ -112,6 +131,15 @@ __device__ __forceinline__ void tld32(uint32_t at, float (&r)[32]) {
         "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
       : "r"(at));
 }
+__device__ __forceinline__ void tld16(uint32_t at, float (&r)[16]) {
+  uint32_t *u = reinterpret_cast<uint32_t *>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+      : "r"(at));
+}
 __device__ __forceinline__ void tld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tst_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tst16(uint32_t at, const uint32_t (&r)[16]) {
@@ -121,18 +149,6 @@ __device__ __forceinline__ void tst16(uint32_t at, const uint32_t (&r)[16]) {
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(at)
       : "memory");
 }
-__device__ __forceinline__ void tst32(uint32_t at, const float (&f)[32]) {
-  const uint32_t *r = reinterpret_cast<const uint32_t *>(f);
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-      "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
-      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(at)
-      : "memory");
-}
-
 // Two f32 operations in one instruction.
 struct F2 {
   uint64_t v;
@@ -191,35 +207,21 @@ __device__ __forceinline__ uint2 widen4(uint32_t w) {
 }
 
 // The ring's order of slots: K(0), then K(j), V(j - 1) for each further block, then V(last).
-struct Walk {
-  int j, c;       // block, slot of it
+template <int KC, int VC>
+struct SlotAt {
+  int j, c;
   bool v;
-  int nb, kc, vc;
-  __device__ __forceinline__ Walk(int nb_, int kc_, int vc_) : j(0), c(0), v(false), nb(nb_), kc(kc_), vc(vc_) {}
-  __device__ __forceinline__ void next() {
-    c++;
-    if (!v && c == kc) {
-      c = 0;
-      if (j == 0) {
-        if (nb == 1)
-          v = true;
-        else
-          j = 1;
-      } else {
-        v = true;
-        j--;
-      }
-    } else if (v && c == vc) {
-      c = 0;
-      if (j == nb - 1) {
-        j = nb;   // done
-      } else if (j == nb - 2) {
-        j = nb - 1;   // V of the last block follows V of the one before it
-      } else {
-        j += 2;
-        v = false;
-      }
+  __device__ __forceinline__ SlotAt(int i, int nb) {
+    if (i < KC) {
+      j = 0;
+      c = i;
+      v = false;
+      return;
     }
+    const int q = (i - KC) / (KC + VC), r = (i - KC) % (KC + VC);
+    v = q + 1 == nb || r >= KC;
+    j = v ? q : q + 1;
+    c = v && q + 1 < nb ? r - KC : r;
   }
 };
 
@@ -253,50 +255,50 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
 
   extern __shared__ __align__(1024) uint8_t csm_raw[];
   uint8_t *csm = csm_raw + ((1024 - (smem_u32(csm_raw) & 1023)) & 1023);
-  float *sc = reinterpret_cast<float *>(csm + S::SC_OFF);
+  BlockInfo *info = reinterpret_cast<BlockInfo *>(csm + S::SC_OFF);
   uint64_t *full = reinterpret_cast<uint64_t *>(csm + S::BAR_OFF);
   uint64_t *empty = full + S::NS, *s_full = empty + S::NS, *p_ready = s_full + 2, *pv_done = p_ready + 2;
-  uint64_t *sc_full = pv_done + 1, *sc_free = sc_full + NSC, *end = sc_free + NSC;
+  uint64_t *info_full = pv_done + 1, *info_free = info_full + NSC, *end = info_free + NSC;
   uint32_t *tslot = reinterpret_cast<uint32_t *>(end + 1);
   int *failed = reinterpret_cast<int *>(tslot + 1);
   __shared__ uint32_t bad_v[4][4];   // bf16 pages: positions of boundary blocks whose V is not finite
-  __shared__ float q_scale[128];
+  __shared__ float q_scale[128], row_top[2][2][128];
   auto slot = [&](int i) { return csm + S::Q_BYTES + i * SLOT; };
   const Pool &p = a.pool;
 
   if (t == 0) {
     for (int i = 0; i < S::NS; i++) {
-      mbar_init(&full[i], kProducers / 32);
+      mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; i++) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_ready[i], kSoftmax / 32);
+      mbar_init(&p_ready[i], kSoftWarps);
     }
     mbar_init(pv_done, 1);
     for (int i = 0; i < NSC; i++) {
-      mbar_init(&sc_full[i], 4);
-      mbar_init(&sc_free[i], kSoftmax / 32);
+      mbar_init(&info_full[i], 1);
+      mbar_init(&info_free[i], kSoftWarps + S::VC);
     }
     mbar_init(end, 1);
     mbar_fence_init();
     *failed = 0;
   }
   if (t < 16) (&bad_v[0][0])[t] = 0;
-  if (warp == 12) {
+  if (warp == kMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tslot)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
 
   // ---- Q into K-major slots, one warp a row, four rows of loads in flight. 8-bit pages: f16 scaled
   // by a power of two per row, so that the row's greatest value lies in 2^8 .. 2^9.
-  if (warp < 12) {
+  {
     constexpr int LD = HD == 512 ? 2 : 1, ACT = HD / 8 < 32 ? HD / 8 : 32;
-    for (int r0 = warp; r0 < 128; r0 += 48) {
+    for (int r0 = warp; r0 < 128; r0 += 64) {
       uint4 in[4][LD];
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        const int r = r0 + 12 * k;
+        const int r = r0 + 16 * k;
 #pragma unroll
         for (int i = 0; i < LD; i++) {
           in[k][i] = make_uint4(0, 0, 0, 0);
@@ -308,8 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
       }
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        const int r = r0 + 12 * k;
-        if (r >= 128) break;
+        const int r = r0 + 16 * k;
         int e = 0;
         if (HALF) {
           uint32_t top = 0;
@@ -350,185 +351,123 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
   const uint32_t tmem = *tslot;
   const uint32_t t_s[2] = {tmem, tmem + 128}, t_o = tmem + 256;
 
-  if (warp >= 4 && warp < 12) {
+  if (warp >= kSoftWarps && warp < kSoftWarps + S::PW) {
     // ============================================================ producers
-    const int pt = t - kSoftmax;
-    constexpr int RPT = HALF ? 2 : 4;                  // rows of a slot a thread moves 16 bytes of
-    constexpr int STEP = HALF ? 64 : 32;
-    const int r0 = HALF ? pt >> 2 : pt >> 3, x = HALF ? pt & 3 : pt & 7;
-    const int32_t *table = a.table + (long long)b * a.table_stride;
-    // Row of the pool that holds position pos (for this KV head), -1 for none.
-    auto page_of = [&](int pos) -> int {
-      if (pos < rt.tlo || pos >= rt.thi) return -2;
-      const int pg = table[pos / p.page_size];
-      return pg;
-    };
-    auto row_of = [&](int pos, int pg) -> long long {
-      if (pg == -2) return -1;
-      if (pg < 0 || pg >= p.n_pages) {
-        paged_raise(a.err, G4_PAGED_BAD_PAGE);
-        return -1;
-      }
-      return ((long long)pg * p.kv_heads + kvh) * p.page_size + pos % p.page_size;
-    };
-    long long cur[RPT], prev[RPT];
-    int pg[RPT];
-#pragma unroll
-    for (int i = 0; i < RPT; i++) {
-      cur[i] = prev[i] = -1;
-      pg[i] = nb > 0 ? page_of(j0 * BN + r0 + STEP * i) : -2;
-    }
-    // This thread's position for the scales (the first four warps), one block ahead.
-    const bool scaler = pt < BN;
-    float nks = 0.0f, nvs = -1.0f;
-    int npg = -2;
-    auto load_scale = [&](int j, int page) {
-      const int pos = (j0 + j) * BN + pt;
-      const long long row = row_of(pos, page);
-      nks = 0.0f;
-      nvs = -1.0f;   // not a scale: no row may see this position
-      if (row >= 0) {
-        nks = HALF ? __ldg(p.ks + row) : 1.0f;
-        nvs = HALF ? __ldg(p.vs + row) : 1.0f;
-      }
-    };
-    if (scaler && nb > 0) {
-      load_scale(0, page_of(j0 * BN + pt));
-      npg = nb > 1 ? page_of((j0 + 1) * BN + pt) : -2;
-    }
-    constexpr int A = S::AHEAD;
-    uint4 st[HALF ? A : 1][RPT];
-    Walk ld(nb, S::KC, S::VC), put(nb, S::KC, S::VC);
+    constexpr int ROW = HALF ? HD : 2 * HD;   // bytes of a position
+    const int total = nb * (S::KC + S::VC), w = warp - kSoftWarps;
     bool ok = true;
-
-    // Loads of the slot `ld` stands at, into register stage k (8 bit) or ring slot n (16 bit).
-    auto load = [&](uint4 (&d)[RPT], int n) {
-      if (!ld.v && ld.c == 0) {
+    // The block's rows are known, or a wait gave up.
+    auto known = [&](const SlotAt<S::KC, S::VC> &at) {
+      return warp_wait(&info_full[at.j % NSC], (uint32_t)((at.j / NSC) & 1));
+    };
+    // This warp's last use of a V slot's rows.
+    auto used = [&](const SlotAt<S::KC, S::VC> &at) {
+      __syncwarp();
+      if (at.v && lane == 0) arrive(&info_free[at.j % NSC]);
+    };
+    auto slot_free = [&](int i) { return i < S::NS || warp_wait(&empty[i % S::NS], (uint32_t)((i / S::NS - 1) & 1)); };
+    auto edge = [&](int j) {
+      const int pos0 = (j0 + j) * BN;
+      return pos0 < rt.all_lo || pos0 + BN > rt.all_hi;
+    };
+    auto in_range = [&](int pos) { return pos >= rt.tlo && pos < rt.thi; };
+    if constexpr (HALF) {
+      // Piece k of a lane: 16 codes of row 8 k + lane / 4.
+      const int rr = lane >> 2, x = lane & 3;
+      uint4 d[16];
+      auto load = [&](uint4 &to, const SlotAt<S::KC, S::VC> &at, const uint8_t *base, int k, bool partly) {
+        const long long row = info[at.j % NSC].at[k >> 1];
+        const bool on = row >= 0 && (!partly || in_range((j0 + at.j) * BN + 8 * k + rr));
+        to = on ? __ldg(reinterpret_cast<const uint4 *>(base + row + (k & 1) * 8 * ROW)) : make_uint4(0, 0, 0, 0);
+      };
+      auto base_of = [&](const SlotAt<S::KC, S::VC> &at) {
+        return (at.v ? p.v + half * S::OD : p.k) + at.c * 64 + rr * ROW + x * 16;
+      };
+      const uint32_t o0 = rr * 128 + (((2 * x) ^ rr) << 4), o1 = o0 ^ 16;
+      if (w < total) {
+        const SlotAt<S::KC, S::VC> at(w, nb);
+        ok = known(at);
+        if (ok) {
+          const uint8_t *base = base_of(at);
+          const bool partly = edge(at.j);
 #pragma unroll
-        for (int i = 0; i < RPT; i++) {
-          prev[i] = cur[i];
-          cur[i] = row_of((j0 + ld.j) * BN + r0 + STEP * i, pg[i]);
-          pg[i] = ld.j + 1 < nb ? page_of((j0 + ld.j + 1) * BN + r0 + STEP * i) : -2;
+          for (int k = 0; k < 16; k++) load(d[k], at, base, k, partly);
+          used(at);
         }
       }
-      const bool latest = ld.j == nb - 1;   // V of the last block: no K moved `cur` on
-      const uint8_t *base = ld.v ? p.v : p.k;
-      const int ch = ld.v ? half * S::VC + ld.c : ld.c;
+#pragma unroll 1
+      for (int i = w; i < total && ok; i += S::PW) {
+        const bool more = i + S::PW < total;
+        const SlotAt<S::KC, S::VC> next(more ? i + S::PW : i, nb);
+        ok = slot_free(i) && (!more || known(next));
+        if (!ok) break;
+        const uint8_t *base = base_of(next);
+        const bool partly = edge(next.j);
+        uint8_t *to = slot(i % S::NS);
 #pragma unroll
-      for (int i = 0; i < RPT; i++) {
-        const long long row = ld.v && !latest ? prev[i] : cur[i];
-        if (HALF) {
-          d[i] = make_uint4(0, 0, 0, 0);
-          if (row >= 0) d[i] = __ldg(reinterpret_cast<const uint4 *>(base + row * HD + ch * 64 + x * 16));
-        } else {
-          const int r = r0 + STEP * i;
-          uint8_t *dst = slot(n) + r * 128 + ((x ^ (r & 7)) << 4);
-          if (row >= 0)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)),
-                         "l"(base + (row * HD + ch * 64) * 2 + x * 16)
-                         : "memory");
+        for (int k = 0; k < 16; k++) {
+          const uint2 w0 = widen4<FMT>(d[k].x), w1 = widen4<FMT>(d[k].y), w2 = widen4<FMT>(d[k].z), w3 = widen4<FMT>(d[k].w);
+          *reinterpret_cast<uint4 *>(to + o0 + k * 1024) = make_uint4(w0.x, w0.y, w1.x, w1.y);
+          *reinterpret_cast<uint4 *>(to + o1 + k * 1024) = make_uint4(w2.x, w2.y, w3.x, w3.y);
+          if (more) load(d[k], next, base, k, partly);
+        }
+        fence_async();
+        __syncwarp();
+        if (lane == 0) arrive(&full[i % S::NS]);
+        if (more) used(next);
+      }
+    } else {
+      // Piece k of a lane: 8 values of row 4 k + lane / 8.
+      const int rr = lane >> 3, x = lane & 7;
+#pragma unroll 1
+      for (int i = w; i < total; i += S::PW) {
+        const SlotAt<S::KC, S::VC> at(i, nb);
+        ok = known(at) && slot_free(i);
+        if (!ok) break;
+        const uint8_t *base = (at.v ? p.v + half * S::OD * 2 : p.k) + at.c * 128 + rr * ROW + x * 16;
+        const bool partly = edge(at.j);
+        const long long *rows = info[at.j % NSC].at;
+        uint8_t *to = slot(i % S::NS);
+#pragma unroll 8
+        for (int k = 0; k < 32; k++) {
+          const int r = 4 * k + rr;
+          const long long row = rows[k >> 2];
+          uint8_t *dst = to + r * 128 + ((x ^ (r & 7)) << 4);
+          if (row >= 0 && (!partly || in_range((j0 + at.j) * BN + r)))
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(base + row + (k & 3) * 4 * ROW) : "memory");
           else
             *reinterpret_cast<uint4 *>(dst) = make_uint4(0, 0, 0, 0);
         }
-      }
-      ld.next();
-    };
-    // Hands slot n over (writing it first from the register stage at 8 bits).
-    auto hand = [&](const uint4 (&d)[RPT], int n) {
-      if constexpr (HALF) {
-#pragma unroll
-        for (int i = 0; i < RPT; i++) {
-          const int r = r0 + STEP * i;
-          const uint2 w0 = widen4<FMT>(d[i].x), w1 = widen4<FMT>(d[i].y), w2 = widen4<FMT>(d[i].z), w3 = widen4<FMT>(d[i].w);
-          uint8_t *row = slot(n) + r * 128;
-          *reinterpret_cast<uint4 *>(row + (((2 * x) ^ (r & 7)) << 4)) = make_uint4(w0.x, w0.y, w1.x, w1.y);
-          *reinterpret_cast<uint4 *>(row + (((2 * x + 1) ^ (r & 7)) << 4)) = make_uint4(w2.x, w2.y, w3.x, w3.y);
-        }
-      } else if (put.v) {
-        // Blocks that some row sees only in part: a weight of 0 must not meet an infinity or a NaN.
-        const int pos0 = (j0 + put.j) * BN;
-        if (pos0 < rt.all_lo || pos0 + BN > rt.all_hi) {
-#pragma unroll
-          for (int i = 0; i < RPT; i++) {
-            const int r = r0 + STEP * i;
-            uint4 *at = reinterpret_cast<uint4 *>(slot(n) + r * 128 + ((x ^ (r & 7)) << 4));
-            uint32_t w[4] = {at->x, at->y, at->z, at->w};
+        used(at);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (at.v && partly) {
+          // A block that some row sees only in part: a weight of 0 must not meet an infinity or a NaN.
+#pragma unroll 1
+          for (int k = 0; k < 32; k++) {
+            const int r = 4 * k + rr;
+            uint4 *q = reinterpret_cast<uint4 *>(to + r * 128 + ((x ^ (r & 7)) << 4));
+            uint32_t u[4] = {q->x, q->y, q->z, q->w};
             bool bad = false;
 #pragma unroll
             for (int z = 0; z < 4; z++) {
-              if ((w[z] & 0x7f80u) == 0x7f80u) {
-                w[z] &= 0xffff0000u;
+              if ((u[z] & 0x7f80u) == 0x7f80u) {
+                u[z] &= 0xffff0000u;
                 bad = true;
               }
-              if ((w[z] & 0x7f800000u) == 0x7f800000u) {
-                w[z] &= 0xffffu;
+              if ((u[z] & 0x7f800000u) == 0x7f800000u) {
+                u[z] &= 0xffffu;
                 bad = true;
               }
             }
             if (bad) {
-              *at = make_uint4(w[0], w[1], w[2], w[3]);
-              atomicOr(&bad_v[put.j < 2 ? put.j : 2 + (nb - 1 - put.j)][r >> 5], 1u << (r & 31));
+              *q = make_uint4(u[0], u[1], u[2], u[3]);
+              atomicOr(&bad_v[at.j < 2 ? at.j : 2 + (nb - 1 - at.j)][r >> 5], 1u << (r & 31));
             }
           }
         }
-      }
-      fence_async();
-      __syncwarp();
-      if (lane == 0) arrive(&full[n]);
-      if (!put.v && put.c == 0 && scaler) {
-        // The block's scales, and the next block's on their way.
-        const int k = put.j % NSC;
-        if (put.j >= NSC && !warp_wait(&sc_free[k], (uint32_t)((put.j / NSC - 1) & 1))) ok = false;
-        float *f = sc + k * 3 * BN;
-        f[pt] = nks;
-        f[BN + pt] = nvs;
-        f[2 * BN + pt] = HALF ? __log2f(fmaxf(nvs, 0x1p-100f)) : 0.0f;
+        fence_async();
         __syncwarp();
-        if (lane == 0) arrive(&sc_full[k]);
-        if (put.j + 1 < nb) {
-          load_scale(put.j + 1, npg);
-          npg = put.j + 2 < nb ? page_of((j0 + put.j + 2) * BN + pt) : -2;
-        }
-      }
-      put.next();
-    };
-
-    const int total = nb * (S::KC + S::VC);
-    if constexpr (HALF) {
-#pragma unroll
-      for (int k = 0; k < A; k++)
-        if (k < total) load(st[k], 0);
-      for (int n = 0; n < total && ok; n += A) {
-#pragma unroll
-        for (int k = 0; k < A; k++) {
-          const int i = n + k;
-          if (i >= total) break;
-          const int sl = i % S::NS;
-          if (i >= S::NS && !warp_wait(&empty[sl], (uint32_t)((i / S::NS - 1) & 1))) {
-            ok = false;
-            break;
-          }
-          hand(st[k], sl);
-          if (i + A < total) load(st[k], 0);
-        }
-      }
-    } else {
-      // Slot i + A - 1 is requested before slot i is handed over: A groups in flight at most.
-      uint4 none[RPT];
-      for (int i = 0; i < total + A - 1 && ok; i++) {
-        if (i < total) {
-          const int sl = i % S::NS;
-          if (i >= S::NS && !warp_wait(&empty[sl], (uint32_t)((i / S::NS - 1) & 1))) {
-            ok = false;
-            break;
-          }
-          load(none, sl);
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (i >= A - 1) {
-          asm volatile("cp.async.wait_group %0;" ::"n"(A - 1) : "memory");
-          hand(none, (i - (A - 1)) % S::NS);
-        }
+        if (lane == 0) arrive(&full[i % S::NS]);
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
     }
@@ -536,36 +475,99 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
       *failed = 1;
       paged_raise(a.err, G4_PAGED_TIMEOUT);
     }
-  } else if (warp == 12) {
+  } else if (warp == kScout) {
+    // ============================================================ the scout: lane l positions 4 l .. + 3
+    const int32_t *table = a.table + (long long)b * a.table_stride;
+    // The page of this lane's 16 positions, -2 where no row sees any of them.
+    auto page_of = [&](int j) -> int {
+      const int pos = (j0 + j) * BN + (lane >> 2) * 16;
+      return j < nb && pos + 16 > rt.tlo && pos < rt.thi ? table[pos / p.page_size] : -2;
+    };
+    int page = page_of(0), next = page_of(1);
+    bool ok = true;
+    for (int j = 0; j < nb; j++) {
+      const int k = j % NSC, pos = (j0 + j) * BN + (lane >> 2) * 16;
+      long long row = -1;
+      if (page >= 0 && page < p.n_pages)
+        row = ((long long)page * p.kv_heads + kvh) * p.page_size + pos % p.page_size;
+      else if (page != -2)
+        paged_raise(a.err, G4_PAGED_BAD_PAGE);
+      page = next;
+      next = page_of(j + 2);
+      const float none = row >= 0 ? 1.0f : -1.0f;
+      float4 ks = make_float4(1, 1, 1, 1), vs = make_float4(none, none, none, none);
+      if (HALF && row >= 0) {
+        ks = __ldg(reinterpret_cast<const float4 *>(p.ks + row + (lane & 3) * 4));
+        vs = __ldg(reinterpret_cast<const float4 *>(p.vs + row + (lane & 3) * 4));
+      }
+      float4 lv = make_float4(0, 0, 0, 0);
+      if (HALF)
+        lv = make_float4(__log2f(fmaxf(vs.x, 0x1p-100f)), __log2f(fmaxf(vs.y, 0x1p-100f)), __log2f(fmaxf(vs.z, 0x1p-100f)),
+                         __log2f(fmaxf(vs.w, 0x1p-100f)));
+      float hi_ = fmaxf(fmaxf(lv.x, lv.y), fmaxf(lv.z, lv.w)), lo_ = fminf(fminf(lv.x, lv.y), fminf(lv.z, lv.w));
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        hi_ = fmaxf(hi_, __shfl_xor_sync(0xffffffffu, hi_, d));
+        lo_ = fminf(lo_, __shfl_xor_sync(0xffffffffu, lo_, d));
+      }
+      const bool even = __all_sync(0xffffffffu, row >= 0) && hi_ - lo_ <= 8.0f;
+      if (j >= NSC) ok = warp_wait(&info_free[k], (uint32_t)((j / NSC - 1) & 1));
+      if (!ok) break;
+      BlockInfo &f = info[k];
+      reinterpret_cast<float4 *>(f.ks)[lane] = ks;
+      reinterpret_cast<float4 *>(f.vs)[lane] = vs;
+      reinterpret_cast<float4 *>(f.lv)[lane] = lv;
+      if ((lane & 3) == 0) f.at[lane >> 2] = row >= 0 ? row * (HALF ? HD : 2 * HD) : -1;
+      if (lane == 0) {
+        f.lmax = hi_;
+        f.even = even;
+      }
+      __syncwarp();
+      if (lane == 0) arrive(&info_full[k]);
+    }
+    if (!ok) {
+      *failed = 1;
+      paged_raise(a.err, G4_PAGED_TIMEOUT);
+    }
+  } else if (warp == kMma) {
     // ============================================================ products
     if (lane == 0) {
       constexpr uint32_t IS = idesc_f16(HALF, BN, false), IO = idesc_f16(HALF, 64, true);
-      int n = 0;
+      int sl = 0;
+      uint32_t round = 0;
       bool ok = true;
+      auto advance = [&] {
+        commit(&empty[sl]);
+        if (++sl == S::NS) {
+          sl = 0;
+          round ^= 1;
+        }
+      };
       auto scores = [&](int j) {
         if (j >= 2 && !mbar_wait(pv_done, (uint32_t)(j & 1))) return false;   // O(j - 2) has read P from these columns
-        for (int c = 0; c < S::KC; c++, n++) {
-          const int sl = n % S::NS;
-          if (!mbar_wait(&full[sl], (uint32_t)((n / S::NS) & 1))) return false;
+#pragma unroll 1
+        for (int c = 0; c < S::KC; c++) {
+          if (!mbar_wait(&full[sl], round)) return false;
           fence_after();
           const uint64_t ad = slot_desc(csm + c * SLOT), bd = slot_desc(slot(sl));
 #pragma unroll
           for (int k = 0; k < 4; k++) mma_ss(t_s[j & 1], ad + 2 * k, bd + 2 * k, IS, (c | k) != 0);
-          commit(&empty[sl]);
+          advance();
         }
         commit(&s_full[j & 1]);
         return true;
       };
       auto outputs = [&](int j) {
         if (!mbar_wait(&p_ready[j & 1], (uint32_t)((j >> 1) & 1))) return false;
-        for (int c = 0; c < S::VC; c++, n++) {
-          const int sl = n % S::NS;
-          if (!mbar_wait(&full[sl], (uint32_t)((n / S::NS) & 1))) return false;
+#pragma unroll 1
+        for (int c = 0; c < S::VC; c++) {
+          if (!mbar_wait(&full[sl], round)) return false;
           fence_after();
           const uint64_t bd = slot_desc(slot(sl));
 #pragma unroll
-          for (int k = 0; k < BN / 16; k++) mma_ts(t_o + 64 * c, t_s[j & 1] + 8 * k, bd + 128 * k, IO, (j | k) != 0);
-          commit(&empty[sl]);
+          for (int k = 0; k < BN / 16; k++)   // P of positions 64 .. lies over their S, from column 64
+            mma_ts(t_o + 64 * c, t_s[j & 1] + 8 * k + (k >= 4 ? 32 : 0), bd + 128 * k, IO, (j | k) != 0);
+          advance();
         }
         commit(pv_done);
         return true;
@@ -588,147 +590,123 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
   float m = -INFINITY, l = 0.0f;
   int lo = 0, hi = 0;
   const float bits = HALF ? 14.0f : 0.0f;
-  const uint32_t lane_base = (uint32_t)(32 * warp) << 16;
-  if (warp < 4) {
-    // ============================================================ softmax: thread t is row t
-    const float qf = q_scale[t];
-    if (t < rt.rows) row_range(a, s.pos + rt.row0 + t / a.group, s.kv, lo, hi);
+  const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
+  const int row = 32 * (warp & 3) + lane, ch = (warp >> 2) & 1;   // softmax: thread's row, its half of the columns
+  if (warp < kSoftWarps) {
+    // ============================================================ softmax
+    const float qf = q_scale[row];
+    if (row < rt.rows) row_range(a, s.pos + rt.row0 + row / a.group, s.kv, lo, hi);
     bool ok = true;
-    for (int j = 0; j < nb && ok; j++) {
-      const int k = j % NSC, pos0 = (j0 + j) * BN;
-      ok = warp_wait(&sc_full[k], (uint32_t)((j / NSC) & 1)) && warp_wait(&s_full[j & 1], (uint32_t)((j >> 1) & 1));
-      if (!ok) break;
-      fence_after();
-      const float4 *ks = reinterpret_cast<const float4 *>(sc + k * 3 * BN), *vs = ks + BN / 4, *lv = vs + BN / 4;
-      const uint32_t at = t_s[j & 1] + lane_base;
-      // Scales within a factor of 2^8 of each other (and every page there): one bound serves them.
-      const float4 mine = lv[lane];
-      const float4 mv = vs[lane];
-      float lmax = fmaxf(fmaxf(mine.x, mine.y), fmaxf(mine.z, mine.w)), lmin = fminf(fminf(mine.x, mine.y), fminf(mine.z, mine.w));
-      float vmin = fminf(fminf(mv.x, mv.y), fminf(mv.z, mv.w));
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        if (HALF) {
-          lmax = fmaxf(lmax, __shfl_xor_sync(0xffffffffu, lmax, d));
-          lmin = fminf(lmin, __shfl_xor_sync(0xffffffffu, lmin, d));
-        }
-        vmin = fminf(vmin, __shfl_xor_sync(0xffffffffu, vmin, d));
-      }
-      const bool plain = pos0 >= rt.all_lo && pos0 + BN <= rt.all_hi && !(vmin < 0.0f) && lmax - lmin <= 8.0f;
-      float top = -INFINITY;
-      float sv[32];
-      if (plain) {
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          tld32(at + 32 * c, sv);
-          tld_wait();
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            if (HALF) {
-              const float4 f = ks[8 * c + i];
-              const float2 u = un2(mul2(f2(sv[4 * i], sv[4 * i + 1]), f2(f.x, f.y)));
-              const float2 w = un2(mul2(f2(sv[4 * i + 2], sv[4 * i + 3]), f2(f.z, f.w)));
-              // A negative scale turns the order round.
-              top = qf >= 0.0f ? max3(top, u.x, u.y) : max3(top, -u.x, -u.y);
-              top = qf >= 0.0f ? max3(top, w.x, w.y) : max3(top, -w.x, -w.y);
-            } else {
-              const float sg = qf >= 0.0f ? 1.0f : -1.0f;
-              top = max3(top, sg * sv[4 * i], sg * sv[4 * i + 1]);
-              top = max3(top, sg * sv[4 * i + 2], sg * sv[4 * i + 3]);
-            }
-          }
-        }
-        top = top * fabsf(qf) + (HALF ? lmax : 0.0f);
-      } else {
 #pragma unroll 1
-        for (int c = 0; c < 4; c++) {
-          tld32(at + 32 * c, sv);
-          tld_wait();
+    for (int j = 0; j < nb; j++) {
+      const int k = j % NSC, pos0 = (j0 + j) * BN + 64 * ch;
+      const auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory"); };
+      ok = ok && warp_wait(&info_full[k], (uint32_t)((j / NSC) & 1)) && warp_wait(&s_full[j & 1], (uint32_t)((j >> 1) & 1));
+      if (!ok) {   // the other half's warp still counts on this one's barriers
+        pair_sync();
+        continue;
+      }
+      fence_after();
+      const BlockInfo &f = info[k];
+      const float4 *ks = reinterpret_cast<const float4 *>(f.ks + 64 * ch), *vs = reinterpret_cast<const float4 *>(f.vs + 64 * ch);
+      const uint32_t at = t_s[j & 1] + lane_base + 64 * ch;
+      const bool plain = (j0 + j) * BN >= rt.all_lo && (j0 + j + 1) * BN <= rt.all_hi && f.even;
+      float z[2][32];
+      tld32(at, z[0]);
+      tld32(at + 32, z[1]);
+      tld_wait();
+      // The scores in units of log2, less the row's factor in the plain case.
+      float top = -INFINITY;
+      if (plain) {
+        const float sg = qf >= 0.0f ? 1.0f : -1.0f;   // a negative scale turns the order round
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            if (HALF) {
+              const float4 c = ks[8 * h + i / 4];
+              const float2 u = un2(mul2(f2(z[h][i], z[h][i + 1]), f2(c.x, c.y)));
+              const float2 w = un2(mul2(f2(z[h][i + 2], z[h][i + 3]), f2(c.z, c.w)));
+              z[h][i] = u.x;
+              z[h][i + 1] = u.y;
+              z[h][i + 2] = w.x;
+              z[h][i + 3] = w.y;
+            }
+            top = max3(top, sg * z[h][i], sg * z[h][i + 1]);
+            top = max3(top, sg * z[h][i + 2], sg * z[h][i + 3]);
+          }
+        top = top * fabsf(qf) + (HALF ? f.lmax : 0.0f);
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
 #pragma unroll
           for (int i = 0; i < 32; i++) {
-            const int q = 32 * c + i, pos = pos0 + q;
-            const float v = reinterpret_cast<const float *>(vs)[q];
-            const float z = sv[i] * reinterpret_cast<const float *>(ks)[q] * qf + reinterpret_cast<const float *>(lv)[q];
-            if (pos >= lo && pos < hi && !(v < 0.0f)) top = fmaxf(top, z);
+            const int q = 64 * ch + 32 * h + i, pos = pos0 + 32 * h + i;
+            const bool see = pos >= lo && pos < hi && !(f.vs[q] < 0.0f);
+            z[h][i] = see ? z[h][i] * f.ks[q] * qf : -INFINITY;
+            if (see) top = fmaxf(top, z[h][i] + f.lv[q]);
           }
-        }
       }
+      // With the other half of the columns.
+      row_top[j & 1][ch][row] = top;
+      pair_sync();
+      top = fmaxf(top, row_top[j & 1][ch ^ 1][row]);
       // The maximum moves only when a row outgrows it by more than 2^1.9.
-      const bool grow = top > m + 1.9f || (m == -INFINITY && top > -INFINITY);
+      const bool grow = top > m + 1.9f;
       if (__any_sync(0xffffffffu, grow)) {
-        const float f = grow ? cex2(m - top) : 1.0f;
+        const float e = grow ? cex2(m - top) : 1.0f;
         if (grow) {
           l = m == -INFINITY ? 0.0f : crescale(l, m - top);
           m = top;
         }
         if (j > 0) {
           ok = warp_wait(pv_done, (uint32_t)((j - 1) & 1));
-          if (!ok) break;
+          if (!ok) continue;
           fence_after();
 #pragma unroll 1
           for (int c = 0; c < S::OD / 32; c++) {
-            float o[32];
-            tld32(t_o + lane_base + 32 * c, o);
+            const uint32_t oc = t_o + lane_base + ch * (S::OD / 2) + 16 * c;
+            float o[16];
+            tld16(oc, o);
             tld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; i++) o[i] *= f;
-            tst32(t_o + lane_base + 32 * c, o);
+            for (int i = 0; i < 16; i++) o[i] *= e;
+            tst16(oc, reinterpret_cast<const uint32_t(&)[16]>(o));
           }
-          tst_wait();
         }
       }
       const float r = m == -INFINITY ? 0.0f : m - bits;
       F2 sum = f2(0.0f, 0.0f);
-      if (plain) {
-        const F2 q2 = f2(qf, qf), r2 = f2(-r, -r);
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-          tld32(at + 32 * c, sv);
-          tld_wait();
-          uint32_t pk[16];
+      for (int h = 0; h < 2; h++) {
+        uint32_t pk[16];
+        if (plain) {
+          const F2 q2 = f2(qf, qf), r2 = f2(-r, -r);
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
-            F2 z0 = f2(sv[4 * i], sv[4 * i + 1]), z1 = f2(sv[4 * i + 2], sv[4 * i + 3]);
-            if (HALF) {
-              const float4 f = ks[8 * c + i];
-              z0 = mul2(z0, f2(f.x, f.y));
-              z1 = mul2(z1, f2(f.z, f.w));
-            }
-            const float2 y0 = un2(fma2(z0, q2, r2)), y1 = un2(fma2(z1, q2, r2));
+          for (int i = 0; i < 32; i += 4) {
+            const float2 y0 = un2(fma2(f2(z[h][i], z[h][i + 1]), q2, r2)), y1 = un2(fma2(f2(z[h][i + 2], z[h][i + 3]), q2, r2));
             F2 p0 = f2(cex2(y0.x), cex2(y0.y)), p1 = f2(cex2(y1.x), cex2(y1.y));
             sum = add2(sum, p0);
             sum = add2(sum, p1);
             if (HALF) {
-              const float4 f = vs[8 * c + i];
-              p0 = mul2(p0, f2(f.x, f.y));
-              p1 = mul2(p1, f2(f.z, f.w));
+              const float4 c = vs[8 * h + i / 4];
+              p0 = mul2(p0, f2(c.x, c.y));
+              p1 = mul2(p1, f2(c.z, c.w));
             }
             const float2 w0 = un2(p0), w1 = un2(p1);
-            pk[2 * i] = pack16<HALF>(w0.x, w0.y);
-            pk[2 * i + 1] = pack16<HALF>(w1.x, w1.y);
+            pk[i / 2] = pack16<HALF>(w0.x, w0.y);
+            pk[i / 2 + 1] = pack16<HALF>(w1.x, w1.y);
           }
-          tst16(at + 16 * c, pk);
-        }
-      } else {
-#pragma unroll 1
-        for (int c = 0; c < 4; c++) {
-          tld32(at + 32 * c, sv);
-          tld_wait();
-          uint32_t pk[16];
+        } else {
 #pragma unroll
-          for (int i = 0; i < 32; i++) {
-            const int q = 32 * c + i, pos = pos0 + q;
-            const float v = reinterpret_cast<const float *>(vs)[q];
-            const bool see = pos >= lo && pos < hi && !(v < 0.0f);
-            const float z = sv[i] * reinterpret_cast<const float *>(ks)[q] * qf;
-            const float e = see ? cex2(z - r) : 0.0f;
-            sum = add2(sum, f2(e, 0.0f));
-            sv[i] = see ? e * v : 0.0f;
+          for (int i = 0; i < 32; i += 2) {
+            const float2 v = *reinterpret_cast<const float2 *>(f.vs + 64 * ch + 32 * h + i);
+            const float e0 = cex2(z[h][i] - r), e1 = cex2(z[h][i + 1] - r);
+            sum = add2(sum, f2(e0, e1));
+            pk[i / 2] = pack16<HALF>(z[h][i] == -INFINITY ? 0.0f : e0 * v.x, z[h][i + 1] == -INFINITY ? 0.0f : e1 * v.y);
           }
-#pragma unroll
-          for (int i = 0; i < 16; i++) pk[i] = pack16<HALF>(sv[2 * i], sv[2 * i + 1]);
-          tst16(at + 16 * c, pk);
         }
+        tst16(at + 16 * h, pk);
       }
       const float2 two = un2(sum);
       l += two.x + two.y;
@@ -737,21 +715,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
       __syncwarp();
       if (lane == 0) {
         arrive(&p_ready[j & 1]);
-        arrive(&sc_free[k]);
+        arrive(&info_free[k]);
       }
     }
     if (!ok) {
       *failed = 1;
       paged_raise(a.err, G4_PAGED_TIMEOUT);
     }
+    // The row's sum over both halves of the columns (after the last maximum was read).
+    asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
+    row_top[0][ch][row] = l;
+    asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
+    l += row_top[0][ch ^ 1][row];
   }
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp < 4 && !*failed) {
+  if (warp < kSoftWarps && !*failed) {
     // ============================================================ the rows out
-    const int i = rt.row0 + t / a.group, h = kvh * a.group + t % a.group;
-    if (!HALF && nb > 0 && t < rt.rows) {
+    const int i = rt.row0 + row / a.group, h = kvh * a.group + row % a.group;
+    const bool live = row < rt.rows;
+    if (!HALF && nb > 0 && live) {
       // A row that sees a value which is not finite is not either.
 #pragma unroll 1
       for (int k = 0; k < 16; k++) {
@@ -765,13 +749,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
       }
     }
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    const bool live = t < rt.rows;
-    __nv_bfloat16 *out = reinterpret_cast<__nv_bfloat16 *>(a.out) + (long long)(s.row + i) * a.o_stride + (long long)h * HD + half * S::OD;
+    __nv_bfloat16 *out = reinterpret_cast<__nv_bfloat16 *>(a.out) + (long long)(s.row + i) * a.o_stride + (long long)h * HD + half * S::OD + ch * (S::OD / 2);
 #pragma unroll 1
-    for (int c = 0; c < S::OD / 32; c++) {
+    for (int c = 0; c < S::OD / 64; c++) {
       float o[32];
       if (nb > 0) {
-        tld32(t_o + lane_base + 32 * c, o);
+        tld32(t_o + lane_base + ch * (S::OD / 2) + 32 * c, o);
         tld_wait();
       } else {
 #pragma unroll
@@ -782,21 +765,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
         for (int k = 0; k < 32; k += 8) {
           uint32_t w[4];
 #pragma unroll
-          for (int z = 0; z < 4; z++) {
-            // (An O row whose weights were all 0 is 0.)
-            w[z] = pack16<false>(o[k + 2 * z] * inv, o[k + 2 * z + 1] * inv);
-          }
+          for (int q = 0; q < 4; q++) w[q] = pack16<false>(o[k + 2 * q] * inv, o[k + 2 * q + 1] * inv);
           *reinterpret_cast<uint4 *>(out + 32 * c + k) = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
     }
-    if (live && a.lse && half == 0)
+    if (live && a.lse && half == 0 && ch == 0)
       a.lse[(long long)(s.row + i) * a.heads + h] = m == -INFINITY ? -INFINITY : (m - bits + log2f(l)) * kLn2f;
   }
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  if (warp == kMma) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
 }  // namespace

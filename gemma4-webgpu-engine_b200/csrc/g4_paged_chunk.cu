@@ -9,9 +9,11 @@
 //    the context in blocks of 128 positions. S = Q K^T and O += P V accumulate in tensor memory:
 //    two S buffers of 128 columns and O of 256 fill its 512 columns. P goes back into the columns
 //    of its S as f16 (bf16 pages: bf16) and is the second product's A operand from there.
-//  - K and V pass through one ring of 16 KB slots, each [128 positions][64 dimensions] 16-bit in
-//    the 128-byte swizzle: K-major B operand of the first product, and the same bytes are the
-//    MN-major B operand of the second, so both are written alike. Six producer warps gather the
+//  - K and V pass through one ring of 16 KB slots of 64-dimension columns in the 128-byte swizzle.
+//    A K slot is one column of 128 positions, K-major B operand; a V slot is all columns of 128 / 64
+//    / 32 positions (head_dim 64 / 128 / 256), MN-major B operand with all of O's dimensions as N: a
+//    product of N 64 costs 112 cycles, not the 32 of its share (head_dim 256 by columns took 3,600
+//    cycles a block for O, 8 products of N 256 are 1,024). Both are written alike. Six producer warps gather the
 //    pages' rows, each a slot of its own: 8-bit codes through registers, the next slot's requested
 //    as this one's are widened to f16, bf16 rows by asynchronous copies. A scout warp reads the
 //    page table and the scales blocks ahead.
@@ -43,9 +45,9 @@ constexpr int NSC = 8;             // buffers of what the scout found out about 
 constexpr float kL2e = 1.44269504088896341f, kLn2f = 0.693147180559945309f;
 
 // A block of positions as the scout leaves it: their scales (vs < 0: no page there), log2 of the V
-// scales, the byte offset of each 16 positions' rows in the pool (-1: none), the greatest log2, and
-// whether one bound serves all (every page there, scales within 2^8 of each other).
-struct BlockInfo {
+// scales, the byte offset of each 16 positions' rows in the pool (the pool's first where there is no
+// page: read, never used), the greatest log2, and whether one bound serves all (every page there, scales within 2^8 of each other).
+struct __align__(16) BlockInfo {
   float ks[BN], vs[BN], lv[BN];
   long long at[BN / 16];
   float lmax;
@@ -59,6 +61,7 @@ struct ChunkShape {
   static constexpr int KC = HD / 64;                    // K slots of a block
   static constexpr int OD = HD < 256 ? HD : 256;        // dimensions of O a block accumulates
   static constexpr int VC = OD / 64;                    // V slots of a block
+  static constexpr int TV = BN / VC;                    // positions of a V slot
   static constexpr int NS = HD == 512 ? 5 : 9;          // ring slots
   // Producer warps: warp w fills slots w, w + PW, ... A slot's rounds are told apart by one parity bit, so
   // whoever waits for a round must know that the one before it has ended: PW <= NS gives that, as
@@ -85,6 +88,11 @@ __device__ __forceinline__ float crescale(float l, float d) {
 __device__ __forceinline__ void arrive(uint64_t *bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ bool elect() {
+  uint32_t on;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(on));
+  return on != 0;
+}
 // A whole warp's bounded wait: all lanes agree on its result.
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity));
@@ -97,10 +105,10 @@ __device__ __forceinline__ void commit(uint64_t *bar) {
 }
 // Shared-memory matrix descriptor, 128-byte swizzle, 8-row groups 1024 bytes apart. It serves both
 // uses of a slot: K-major (rows are N, 64 K elements a row) and MN-major (rows are K, 64 N
-// elements a row).
-__device__ __forceinline__ uint64_t slot_desc(const void *p) {
+// elements a row, columns `column` bytes apart).
+__device__ __forceinline__ uint64_t slot_desc(const void *p, uint32_t column = 16) {
   const uint32_t a = smem_u32(p);
-  return (uint64_t)((a >> 4) & 0x3FFF) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+  return (uint64_t)((a >> 4) & 0x3FFF) | ((uint64_t)(column >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 // Instruction descriptor, kind::f16: D f32, A and B f16 or bf16, M 128, N n, B MN-major or not.
 constexpr uint32_t idesc_f16(bool half, int n, bool b_mn) {
@@ -293,6 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
   // ---- Q into K-major slots, one warp a row, four rows of loads in flight. 8-bit pages: f16 scaled
   // by a power of two per row, so that the row's greatest value lies in 2^8 .. 2^9.
   {
+    const uint32_t flip = __float_as_uint(a.scale) & 0x80000000u;   // a negative scale turns Q round: row factors are >= 0
     constexpr int LD = HD == 512 ? 2 : 1, ACT = HD / 8 < 32 ? HD / 8 : 32;
     for (int r0 = warp; r0 < 128; r0 += 64) {
       uint4 in[4][LD];
@@ -325,11 +334,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
           e = (int)(top >> 7) - 127;
           e = e < -110 ? -110 : (e > 127 ? 0 : e);
         }
-        const float f = __uint_as_float((uint32_t)(127 + 8 - e) << 23);
+        const float f = __uint_as_float((uint32_t)(127 + 8 - e) << 23 | flip);
 #pragma unroll
         for (int i = 0; i < LD; i++) {
           uint4 o = in[k][i];
-          if (HALF) {
+          if (!HALF) {
+            const uint32_t two = flip | flip >> 16;
+            o = make_uint4(o.x ^ two, o.y ^ two, o.z ^ two, o.w ^ two);
+          } else {
             uint32_t w[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
             for (int z = 0; z < 4; z++)
@@ -340,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
           if (lane < ACT)
             *reinterpret_cast<uint4 *>(csm + (d >> 6) * SLOT + r * 128 + ((((d >> 3) & 7) ^ (r & 7)) << 4)) = o;
         }
-        if (lane == 0) q_scale[r] = a.scale * kL2e * (HALF ? __uint_as_float((uint32_t)(127 - 8 + e) << 23) : 1.0f);
+        if (lane == 0) q_scale[r] = fabsf(a.scale) * kL2e * (HALF ? __uint_as_float((uint32_t)(127 - 8 + e) << 23) : 1.0f);
       }
     }
     fence_async();
@@ -370,18 +382,42 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
       const int pos0 = (j0 + j) * BN;
       return pos0 < rt.all_lo || pos0 + BN > rt.all_hi;
     };
-    auto in_range = [&](int pos) { return pos >= rt.tlo && pos < rt.thi; };
+    // A block some of whose positions some row may not see, or that lacks a page; and whether a position
+    // of it is there for any row.
+    auto odd_block = [&](int j) { return edge(j) || !info[j % NSC].even; };
+    auto seen = [&](int j, int q) {
+      const int pos = (j0 + j) * BN + q;
+      return pos >= rt.tlo && pos < rt.thi && !(info[j % NSC].vs[q] < 0.0f);
+    };
     if constexpr (HALF) {
-      // Piece k of a lane: 16 codes of row 8 k + lane / 4.
+      // Piece k of a lane: 16 codes of row 8 k + lane / 4 of the slot's columns laid end to end.
       const int rr = lane >> 2, x = lane & 3;
       uint4 d[16];
-      auto load = [&](uint4 &to, const SlotAt<S::KC, S::VC> &at, const uint8_t *base, int k, bool partly) {
-        const long long row = info[at.j % NSC].at[k >> 1];
-        const bool on = row >= 0 && (!partly || in_range((j0 + at.j) * BN + 8 * k + rr));
-        to = on ? __ldg(reinterpret_cast<const uint4 *>(base + row + (k & 1) * 8 * ROW)) : make_uint4(0, 0, 0, 0);
+      // Where pieces 2 k and 2 k + 1 start. (Read together, before the stores to shared memory that they
+      // may not pass.)
+      long long rows[8];
+      auto find = [&](const SlotAt<S::KC, S::VC> &at) {
+        const long long *src = info[at.j % NSC].at;
+        constexpr int T = S::TV / 16;
+#pragma unroll
+        for (int k = 0; k < 8; k++) rows[k] = src[at.v ? at.c * T + k % T : k] + (at.v ? 64 * (k / T) : 0);
       };
+      auto load = [&](const uint8_t *base, int k) {
+        return __ldg(reinterpret_cast<const uint4 *>(base + rows[k >> 1] + (k & 1) * 8 * ROW));
+      };
+      // e4m3 codes of V at positions that no row sees may be NaN, which a weight of 0 would not hide:
+      // the pieces of a slot to set to zero.
+      auto unseen = [&](const SlotAt<S::KC, S::VC> &at) -> uint32_t {
+        uint32_t m = 0;
+        if (FMT == G4_PAGE_E4M3 && at.v && odd_block(at.j)) {
+          for (int k = 0; k < 16; k++)
+            if (!seen(at.j, at.c * S::TV + 8 * (k % (S::TV / 8)) + rr)) m |= 1u << k;
+        }
+        return m;
+      };
+      uint32_t zero = 0;
       auto base_of = [&](const SlotAt<S::KC, S::VC> &at) {
-        return (at.v ? p.v + half * S::OD : p.k) + at.c * 64 + rr * ROW + x * 16;
+        return (at.v ? p.v + half * S::OD : p.k + at.c * 64) + rr * ROW + x * 16;
       };
       const uint32_t o0 = rr * 128 + (((2 * x) ^ rr) << 4), o1 = o0 ^ 16;
       if (w < total) {
@@ -389,9 +425,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
         ok = known(at);
         if (ok) {
           const uint8_t *base = base_of(at);
-          const bool partly = edge(at.j);
+          find(at);
+          zero = unseen(at);
 #pragma unroll
-          for (int k = 0; k < 16; k++) load(d[k], at, base, k, partly);
+          for (int k = 0; k < 16; k++) d[k] = load(base, k);
           used(at);
         }
       }
@@ -402,14 +439,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
         ok = slot_free(i) && (!more || known(next));
         if (!ok) break;
         const uint8_t *base = base_of(next);
-        const bool partly = edge(next.j);
+        if (FMT == G4_PAGE_E4M3 && zero) {
+#pragma unroll
+          for (int k = 0; k < 16; k++)
+            if ((zero >> k) & 1) d[k] = make_uint4(0, 0, 0, 0);
+        }
+        zero = more ? unseen(next) : 0;
         uint8_t *to = slot(i % S::NS);
+        find(next);
 #pragma unroll
         for (int k = 0; k < 16; k++) {
           const uint2 w0 = widen4<FMT>(d[k].x), w1 = widen4<FMT>(d[k].y), w2 = widen4<FMT>(d[k].z), w3 = widen4<FMT>(d[k].w);
           *reinterpret_cast<uint4 *>(to + o0 + k * 1024) = make_uint4(w0.x, w0.y, w1.x, w1.y);
           *reinterpret_cast<uint4 *>(to + o1 + k * 1024) = make_uint4(w2.x, w2.y, w3.x, w3.y);
-          if (more) load(d[k], next, base, k, partly);
+          if (more) d[k] = load(base, k);
         }
         fence_async();
         __syncwarp();
@@ -417,34 +460,34 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
         if (more) used(next);
       }
     } else {
-      // Piece k of a lane: 8 values of row 4 k + lane / 8.
+      // Piece k of a lane: 8 values of row 4 k + lane / 8 of the slot's columns laid end to end.
       const int rr = lane >> 3, x = lane & 7;
 #pragma unroll 1
       for (int i = w; i < total; i += S::PW) {
         const SlotAt<S::KC, S::VC> at(i, nb);
         ok = known(at) && slot_free(i);
         if (!ok) break;
-        const uint8_t *base = (at.v ? p.v + half * S::OD * 2 : p.k) + at.c * 128 + rr * ROW + x * 16;
-        const bool partly = edge(at.j);
+        const uint8_t *base = (at.v ? p.v + half * S::OD * 2 : p.k + at.c * 128) + rr * ROW + x * 16;
+        const bool partly = odd_block(at.j);
         const long long *rows = info[at.j % NSC].at;
         uint8_t *to = slot(i % S::NS);
 #pragma unroll 8
         for (int k = 0; k < 32; k++) {
-          const int r = 4 * k + rr;
-          const long long row = rows[k >> 2];
+          const int r = 4 * k + rr, q = at.v ? at.c * S::TV + 4 * (k % (S::TV / 4)) + rr : r;   // q: position in the block
+          const long long row = rows[q >> 4] + (at.v ? 128 * (k / (S::TV / 4)) : 0);
           uint8_t *dst = to + r * 128 + ((x ^ (r & 7)) << 4);
-          if (row >= 0 && (!partly || in_range((j0 + at.j) * BN + r)))
+          if (!partly || seen(at.j, q))
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(base + row + (k & 3) * 4 * ROW) : "memory");
           else
             *reinterpret_cast<uint4 *>(dst) = make_uint4(0, 0, 0, 0);
         }
         used(at);
         asm volatile("cp.async.wait_all;" ::: "memory");
-        if (at.v && partly) {
+        if (at.v && edge(at.j)) {
           // A block that some row sees only in part: a weight of 0 must not meet an infinity or a NaN.
 #pragma unroll 1
           for (int k = 0; k < 32; k++) {
-            const int r = 4 * k + rr;
+            const int r = 4 * k + rr, pos = at.c * S::TV + 4 * (k % (S::TV / 4)) + rr;
             uint4 *q = reinterpret_cast<uint4 *>(to + r * 128 + ((x ^ (r & 7)) << 4));
             uint32_t u[4] = {q->x, q->y, q->z, q->w};
             bool bad = false;
@@ -461,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
             }
             if (bad) {
               *q = make_uint4(u[0], u[1], u[2], u[3]);
-              atomicOr(&bad_v[at.j < 2 ? at.j : 2 + (nb - 1 - at.j)][r >> 5], 1u << (r & 31));
+              atomicOr(&bad_v[at.j < 2 ? at.j : 2 + (nb - 1 - at.j)][pos >> 5], 1u << (pos & 31));
             }
           }
         }
@@ -517,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
       reinterpret_cast<float4 *>(f.ks)[lane] = ks;
       reinterpret_cast<float4 *>(f.vs)[lane] = vs;
       reinterpret_cast<float4 *>(f.lv)[lane] = lv;
-      if ((lane & 3) == 0) f.at[lane >> 2] = row >= 0 ? row * (HALF ? HD : 2 * HD) : -1;
+      if ((lane & 3) == 0) f.at[lane >> 2] = row >= 0 ? row * (HALF ? HD : 2 * HD) : 0;
       if (lane == 0) {
         f.lmax = hi_;
         f.even = even;
@@ -531,59 +574,71 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
     }
   } else if (warp == kMma) {
     // ============================================================ products
-    if (lane == 0) {
-      constexpr uint32_t IS = idesc_f16(HALF, BN, false), IO = idesc_f16(HALF, 64, true);
-      int sl = 0;
-      uint32_t round = 0;
-      bool ok = true;
-      auto advance = [&] {
-        commit(&empty[sl]);
-        if (++sl == S::NS) {
-          sl = 0;
-          round ^= 1;
-        }
-      };
-      auto scores = [&](int j) {
-        if (j >= 2 && !mbar_wait(pv_done, (uint32_t)(j & 1))) return false;   // O(j - 2) has read P from these columns
+    // The whole warp walks the slots and one elected lane issues: control flow the compiler can see
+    // to be uniform (under a plain lane test each issue took 130 cycles and more). For the same
+    // reason a wait that gave up only shortens the ones after it.
+    constexpr uint32_t IS = idesc_f16(HALF, BN, false), IO = idesc_f16(HALF, S::OD, true);
+    int sl = 0;
+    uint32_t round = 0;
+    bool bad = false;
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+      if (!bad && !mbar_wait(bar, parity)) bad = true;
+    };
+    auto advance = [&] {
+      if (++sl == S::NS) {
+        sl = 0;
+        round ^= 1;
+      }
+    };
+    auto scores = [&](int j) {
+      if (j >= 2) wait(pv_done, (uint32_t)(j & 1));   // O(j - 2) has read P from these columns
 #pragma unroll 1
-        for (int c = 0; c < S::KC; c++) {
-          if (!mbar_wait(&full[sl], round)) return false;
-          fence_after();
-          const uint64_t ad = slot_desc(csm + c * SLOT), bd = slot_desc(slot(sl));
+      for (int c = 0; c < S::KC; c++) {
+        wait(&full[sl], round);
+        fence_after();
+        const uint64_t ad = slot_desc(csm + c * SLOT), bd = slot_desc(slot(sl));
+        if (elect()) {
 #pragma unroll
           for (int k = 0; k < 4; k++) mma_ss(t_s[j & 1], ad + 2 * k, bd + 2 * k, IS, (c | k) != 0);
-          advance();
+          commit(&empty[sl]);
+          if (c == S::KC - 1) commit(&s_full[j & 1]);
         }
-        commit(&s_full[j & 1]);
-        return true;
-      };
-      auto outputs = [&](int j) {
-        if (!mbar_wait(&p_ready[j & 1], (uint32_t)((j >> 1) & 1))) return false;
+        advance();
+      }
+    };
+    auto outputs = [&](int j) {
+      wait(&p_ready[j & 1], (uint32_t)((j >> 1) & 1));
 #pragma unroll 1
-        for (int c = 0; c < S::VC; c++) {
-          if (!mbar_wait(&full[sl], round)) return false;
-          fence_after();
-          const uint64_t bd = slot_desc(slot(sl));
+      for (int c = 0; c < S::VC; c++) {
+        wait(&full[sl], round);
+        fence_after();
+        const uint64_t bd = slot_desc(slot(sl), S::TV * 128);
+        // P of positions 64 .. lies over their S, from column 64.
+        const int q = c * (S::TV / 16);
+        const uint32_t ta = t_s[j & 1] + 8 * q + (S::VC > 1 && q >= 4 ? 32 : 0);
+        if (elect()) {
 #pragma unroll
-          for (int k = 0; k < BN / 16; k++)   // P of positions 64 .. lies over their S, from column 64
-            mma_ts(t_o + 64 * c, t_s[j & 1] + 8 * k + (k >= 4 ? 32 : 0), bd + 128 * k, IO, (j | k) != 0);
-          advance();
+          for (int k = 0; k < S::TV / 16; k++)
+            mma_ts(t_o, ta + 8 * k + (S::VC == 1 && k >= 4 ? 32 : 0), bd + 128 * k, IO, (j | c | k) != 0);
+          commit(&empty[sl]);
+          if (c == S::VC - 1) commit(pv_done);
         }
-        commit(pv_done);
-        return true;
-      };
-      for (int j = 0; j < nb && ok; j++) {
-        ok = scores(j);
-        if (ok && j >= 1) ok = outputs(j - 1);
+        advance();
       }
-      if (ok && nb > 0) ok = outputs(nb - 1);
-      if (!ok) {
-        *failed = 1;
-        paged_raise(a.err, G4_PAGED_TIMEOUT);
-      }
-      // Everything issued has ended before tensor memory and the slots are given up.
-      commit(end);
-      if (!mbar_wait(end, 0)) paged_raise(a.err, G4_PAGED_TIMEOUT);
+    };
+#pragma unroll 1
+    for (int j = 0; j < nb; j++) {
+      scores(j);
+      if (j >= 1) outputs(j - 1);
+    }
+    if (nb > 0) outputs(nb - 1);
+    // Everything issued has ended before tensor memory and the slots are given up.
+    if (elect()) commit(end);
+    __syncwarp();
+    if (!mbar_wait(end, 0)) bad = true;
+    if (bad) {
+      *failed = 1;
+      paged_raise(a.err, G4_PAGED_TIMEOUT);
     }
     __syncwarp();
   }
@@ -618,7 +673,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
       // The scores in units of log2, less the row's factor in the plain case.
       float top = -INFINITY;
       if (plain) {
-        const float sg = qf >= 0.0f ? 1.0f : -1.0f;   // a negative scale turns the order round
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
@@ -632,10 +686,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
               z[h][i + 2] = w.x;
               z[h][i + 3] = w.y;
             }
-            top = max3(top, sg * z[h][i], sg * z[h][i + 1]);
-            top = max3(top, sg * z[h][i + 2], sg * z[h][i + 3]);
+            top = max3(top, z[h][i], z[h][i + 1]);
+            top = max3(top, z[h][i + 2], z[h][i + 3]);
           }
-        top = top * fabsf(qf) + (HALF ? f.lmax : 0.0f);
+        top = top * qf + (HALF ? f.lmax : 0.0f);
       } else {
 #pragma unroll
         for (int h = 0; h < 2; h++)

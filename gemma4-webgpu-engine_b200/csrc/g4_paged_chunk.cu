@@ -62,12 +62,14 @@ struct ChunkShape {
   static constexpr int OD = HD < 256 ? HD : 256;        // dimensions of O a block accumulates
   static constexpr int VC = OD / 64;                    // V slots of a block
   static constexpr int TV = BN / VC;                    // positions of a V slot
-  static constexpr int NS = HD == 512 ? 5 : 9;          // ring slots
+  static constexpr int NS = HD == 512 ? 4 : 8;          // ring slots
+  static constexpr int G = VC;                          // consecutive slots the issue loop is unrolled over
+  static_assert(NS % G == 0 && KC % G == 0, "groups of slots stay whole around the ring");
   // Producer warps: warp w fills slots w, w + PW, ... A slot's rounds are told apart by one parity bit, so
-  // whoever waits for a round must know that the one before it has ended: PW <= NS gives that, as
-  // the warp's own last slot is then consumed no earlier than the slot it waits for was filled.
-  static constexpr int PW = HD == 512 ? 5 : kProdWarps;
-  static_assert(PW == NS || NS >= PW + 3, "see PW");
+  // whoever waits for a round must know that the one before it has begun: slots are consumed in
+  // order, and with PW <= NS the warp's own last slot was filled after that one's consumption.
+  static constexpr int PW = HD == 512 ? 4 : kProdWarps;
+  static_assert(PW <= NS, "see PW");
   static constexpr int Q_BYTES = KC * SLOT;
   static constexpr int SC_OFF = Q_BYTES + NS * SLOT;
   static constexpr int BAR_OFF = SC_OFF + NSC * (int)sizeof(BlockInfo);
@@ -574,71 +576,75 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
     }
   } else if (warp == kMma) {
     // ============================================================ products
-    // The whole warp walks the slots and one elected lane issues: control flow the compiler can see
-    // to be uniform (under a plain lane test each issue took 130 cycles and more). For the same
-    // reason a wait that gave up only shortens the ones after it.
-    constexpr uint32_t IS = idesc_f16(HALF, BN, false), IO = idesc_f16(HALF, S::OD, true);
-    int sl = 0;
-    uint32_t round = 0;
-    bool bad = false;
-    auto wait = [&](uint64_t *bar, uint32_t parity) {
-      if (!bad && !mbar_wait(bar, parity)) bad = true;
-    };
-    auto advance = [&] {
-      if (++sl == S::NS) {
-        sl = 0;
-        round ^= 1;
-      }
-    };
-    auto scores = [&](int j) {
-      if (j >= 2) wait(pv_done, (uint32_t)(j & 1));   // O(j - 2) has read P from these columns
-#pragma unroll 1
-      for (int c = 0; c < S::KC; c++) {
-        wait(&full[sl], round);
-        fence_after();
-        const uint64_t ad = slot_desc(csm + c * SLOT), bd = slot_desc(slot(sl));
-        if (elect()) {
+    // One thread, and the slots of a group unrolled: an issue waits until the products before it are
+    // nearly done, so whatever stands between two issues is lost. (Per block of head_dim 256, whose
+    // products are 2,056 cycles: 2,326 like this, 3,490 with the slots in a loop, 4,490 with the whole
+    // warp waiting and electing at each.)
+    if (elect()) {
+      constexpr uint32_t IS = idesc_f16(HALF, BN, false), IO = idesc_f16(HALF, S::OD, true);
+      const uint64_t q0 = slot_desc(csm), k0 = slot_desc(slot(0)), v0 = slot_desc(slot(0), S::TV * 128);
+      int at = 0;             // the ring's group at hand, in slots, and its round
+      uint32_t round = 0;
+      bool bad = false;       // a wait gave up: the rest is issued without waiting, and not used
+      auto wait = [&](uint64_t *bar, uint32_t parity) {
+        if (!mbar_try_wait(bar, parity) && !bad) bad = !mbar_wait(bar, parity);
+      };
+      auto advance = [&] {
+        at += S::G;
+        if (at == S::NS) {
+          at = 0;
+          round ^= 1;
+        }
+      };
+      auto scores = [&](int j) {
+        const uint32_t d = t_s[j & 1];
+        if (j >= 2) wait(pv_done, (uint32_t)(j & 1));   // O(j - 2) has read P from these columns
 #pragma unroll
-          for (int k = 0; k < 4; k++) mma_ss(t_s[j & 1], ad + 2 * k, bd + 2 * k, IS, (c | k) != 0);
-          commit(&empty[sl]);
-          if (c == S::KC - 1) commit(&s_full[j & 1]);
+        for (int h = 0; h < S::KC / S::G; h++) {
+          const uint64_t kd = k0 + at * (SLOT >> 4);
+#pragma unroll
+          for (int c = 0; c < S::G; c++) {
+            wait(&full[at + c], round);
+            fence_after();
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+              mma_ss(d, q0 + (h * S::G + c) * (SLOT >> 4) + 2 * k, kd + c * (SLOT >> 4) + 2 * k, IS, (h | c | k) != 0);
+            commit(&empty[at + c]);
+          }
+          advance();
+        }
+        commit(&s_full[j & 1]);
+      };
+      auto outputs = [&](int j) {
+        const uint32_t d = t_s[j & 1];
+        const uint64_t vd = v0 + at * (SLOT >> 4);
+        wait(&p_ready[j & 1], (uint32_t)((j >> 1) & 1));
+#pragma unroll
+        for (int c = 0; c < S::VC; c++) {
+          wait(&full[at + c], round);
+          fence_after();
+#pragma unroll
+          for (int k = 0; k < S::TV / 16; k++) {
+            const int q = c * (S::TV / 16) + k;   // P of positions 64 .. lies over their S, from column 64
+            mma_ts(t_o, d + 8 * q + (q >= 4 ? 32 : 0), vd + c * (SLOT >> 4) + 128 * k, IO, (j | q) != 0);
+          }
+          commit(&empty[at + c]);
         }
         advance();
-      }
-    };
-    auto outputs = [&](int j) {
-      wait(&p_ready[j & 1], (uint32_t)((j >> 1) & 1));
+        commit(pv_done);
+      };
 #pragma unroll 1
-      for (int c = 0; c < S::VC; c++) {
-        wait(&full[sl], round);
-        fence_after();
-        const uint64_t bd = slot_desc(slot(sl), S::TV * 128);
-        // P of positions 64 .. lies over their S, from column 64.
-        const int q = c * (S::TV / 16);
-        const uint32_t ta = t_s[j & 1] + 8 * q + (S::VC > 1 && q >= 4 ? 32 : 0);
-        if (elect()) {
-#pragma unroll
-          for (int k = 0; k < S::TV / 16; k++)
-            mma_ts(t_o, ta + 8 * k + (S::VC == 1 && k >= 4 ? 32 : 0), bd + 128 * k, IO, (j | c | k) != 0);
-          commit(&empty[sl]);
-          if (c == S::VC - 1) commit(pv_done);
-        }
-        advance();
+      for (int j = 0; j <= nb; j++) {
+        if (j < nb) scores(j);
+        if (j >= 1) outputs(j - 1);
       }
-    };
-#pragma unroll 1
-    for (int j = 0; j < nb; j++) {
-      scores(j);
-      if (j >= 1) outputs(j - 1);
-    }
-    if (nb > 0) outputs(nb - 1);
-    // Everything issued has ended before tensor memory and the slots are given up.
-    if (elect()) commit(end);
-    __syncwarp();
-    if (!mbar_wait(end, 0)) bad = true;
-    if (bad) {
-      *failed = 1;
-      paged_raise(a.err, G4_PAGED_TIMEOUT);
+      // Everything issued has ended before tensor memory and the slots are given up.
+      commit(end);
+      if (!mbar_wait(end, 0)) bad = true;
+      if (bad) {
+        *failed = 1;
+        paged_raise(a.err, G4_PAGED_TIMEOUT);
+      }
     }
     __syncwarp();
   }

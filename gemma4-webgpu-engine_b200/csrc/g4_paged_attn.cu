@@ -7,20 +7,19 @@
 // products' 16-bit weights keep their precision however far the scales lie apart; the sum of p_t
 // is f32. What bounds the kernel is reading the codes once from HBM (1 byte a value at 8 bits), so
 // everything else has to stay out of the loads' way:
-//  - Codes go from global memory straight into the registers of the matrix products, with no
-//    shared memory between. The sums over head_dim and over positions may run in any order, so
-//    each lane's 16-byte load is taken as it comes: for S^T = K Q^T (16 positions x 8 rows) lane
-//    (g, c) holds 16 codes of positions g and g + 8 as four K steps, for O^T = V^T P^T (16
-//    dimensions x 8 rows) 16 codes of positions 2c, 2c + 1, 2c + 8, 2c + 9, two dimensions a step.
-//    8-bit codes become f16 exactly in two instructions per pair or less; Q is laid out to match,
-//    in shared memory, once.
+//  - The 16 positions of a tile lie side by side in their page (a KV head's rows are contiguous), so
+//    one bulk copy brings all of K's rows, one V's, two the scales. Each group of warps keeps a ring
+//    of such units in flight; nothing but the copy engine waits for memory.
+//  - Codes go from shared memory into the registers of the matrix products as they lie. The sums over
+//    head_dim and over positions may run in any order: for S^T = K Q^T (16 positions x 8 rows) lane
+//    (g, c) takes 16 bytes of positions g and g + 8 as its part of four K steps, for O^T = V^T P^T (16
+//    dimensions x 8 rows) 16 bytes of positions 2c, 2c + 1, 2c + 8, 2c + 9, two dimensions a step. 8-bit
+//    codes become f16 exactly in about an instruction each; Q is laid out to match, once.
 //  - Eight rows fill the N of the products, so a group of 8 heads wastes none of it, and one
 //    8 x 8 transpose in registers turns S^T's layout into P^T's.
-//  - A ring of four 16-register buffers keeps up to three chunks of 2 KB a warp in flight through
-//    the score and the softmax of the chunk at hand.
 //  - f32 rows: q and p vs are carried in two f16 parts (8-bit codes; 22 bits together) or three
 //    bf16 parts (bf16 pages), one product each, all accumulated in f32.
-// The warps of a block take a split's tiles in turn and join through shared memory. A context that
+// The warp groups of a block take a split's tiles in turn and join through shared memory. A context that
 // one block per (sequence, KV head) would leave most SMs idle for is split over blocks; the
 // last of 16 splits to finish joins them, and the last such group joins the groups (one block
 // would read 2.4 MB alone for 148 splits of head_dim 512).
@@ -110,19 +109,23 @@ __device__ __forceinline__ void split2(float v0, float v1, uint32_t (&out)[NP]) 
   }
 }
 
-template <int FMT, int HD, int NP>
+template <int FMT, int HD, int NP, int RT>
 struct DecShape {
   static constexpr bool HALF = FMT != G4_PAGE_BF16;
   static constexpr int ES = HALF ? 1 : 2;              // bytes of a code
   static constexpr int ROW = HD * ES;                  // bytes of a position
   static constexpr bool NARROW = ROW == 64;            // V loads of 8 bytes instead of 16
-  static constexpr int HC = NARROW ? 1 : ROW / 128;    // chunks of K, and of V, per tile
-  static constexpr int C = 2 * HC;
-  static constexpr int NB = 4;                         // ring buffers
-  static constexpr int TILES = C >= NB ? 1 : NB / C;   // tiles per pass of the unrolled loop
   static constexpr int KSTEPS = HD / 16;
-  // Blocks per SM the registers are bounded for: O takes HD / 4 registers, the ring 64.
-  static constexpr int OCC = HD <= 256 ? 3 : 2;
+  static constexpr int TG = kDecWarps / RT;            // groups of warps, a ring each
+  static constexpr int UNIT = 16 * ROW + (HALF ? 128 : 0);   // K's (with both scales) or V's 16 positions
+  static constexpr int Q_BYTES = RT * NP * KSTEPS * 32 * 8;
+  // Two blocks on an SM where three units a ring fit into half of its shared memory.
+  static constexpr int D2 = (108 * 1024 - Q_BYTES) / (TG * UNIT), D1 = (222 * 1024 - Q_BYTES) / (TG * UNIT);
+  static constexpr int OCC = D2 >= 3 ? 2 : 1;
+  static constexpr int DD = OCC == 2 ? D2 : D1, D = DD > 8 ? 8 : DD;
+  static_assert(D >= 2, "a ring holds K and V of a tile");
+  static constexpr int RING = TG * D * UNIT, JOIN = TG * 8 * RT * (HD + 2) * 4;
+  static constexpr int SMEM = Q_BYTES + RING > JOIN ? Q_BYTES + RING : JOIN;
 };
 
 // The join of `np` partials of `rows` rows (o [rows][HD], then m [rows], l [rows] each `stride`
@@ -184,10 +187,10 @@ __device__ __forceinline__ void join_partials(const PagedAttn &a, const float *p
 // Block (row group x KV head, split, sequence): 8 RT rows; RT warps share each tile of positions,
 // one row tile of 8 each, and 4 / RT tiles are worked on side by side.
 template <int FMT, int HD, int NP, int RT>
-__global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP>::OCC) k_paged_decode(const PagedAttn a) {
-  using S = DecShape<FMT, HD, NP>;
+__global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC) k_paged_decode(const PagedAttn a) {
+  using S = DecShape<FMT, HD, NP, RT>;
   constexpr bool HALF = S::HALF;
-  constexpr int TG = kDecWarps / RT, ROWS = 8 * RT;
+  constexpr int TG = S::TG, ROWS = 8 * RT, D = S::D;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, g = lane >> 2, c = lane & 3;
   const int rt = warp % RT, tg = warp / RT;
   const int split = blockIdx.y, rg = blockIdx.x % a.row_groups, kvh = blockIdx.x / a.row_groups, b = blockIdx.z;
@@ -202,7 +205,62 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP>::OCC) k_
   if (split >= ns) return;
   const int tile0 = first + split * a.split_tiles, tile1 = min(last, tile0 + a.split_tiles);
 
-  extern __shared__ __align__(16) uint8_t dsm[];
+  // ---- this group's tiles: tile0 + tg + TG n; its first warp asks for them.
+  const Pool &p = a.pool;
+  const int mine = tile1 - tile0 - tg > 0 ? (tile1 - tile0 - tg + TG - 1) / TG : 0;
+  const int per_page = p.page_size >> 4;
+  const int32_t *table = a.table + (long long)b * a.table_stride;
+  // Lane i of the first warp holds the page of the i-th of 32 tiles from pages_at on (-1: none).
+  int pages = -1, pages_at = 0;
+  auto fetch_pages = [&](int n) {
+    const int k = n + lane;
+    pages = k < mine ? table[(tile0 + tg + TG * k) / per_page] : -1;
+    if (k < mine && (pages < 0 || pages >= p.n_pages)) {
+      paged_raise(a.err, G4_PAGED_BAD_PAGE);
+      pages = -1;
+    }
+    pages_at = n;
+  };
+  if (rt == 0 && mine > 0) fetch_pages(0);
+
+  extern __shared__ __align__(128) uint8_t dsm[];   // Q, then the groups' rings; at the end the groups' partials
+  uint8_t *ring = dsm + S::Q_BYTES + tg * D * S::UNIT;
+  __shared__ uint64_t full_[TG][D], empty_[TG][D];
+  __shared__ int has_[TG][D];   // whether the unit's page exists
+  uint64_t *full = full_[tg], *empty = empty_[tg];
+  volatile int *has = has_[tg];
+  if (t == 0) {
+    for (int i = 0; i < TG * D; i++) {
+      mbar_init(&full_[0][i], 1);
+      mbar_init(&empty_[0][i], RT);
+    }
+    mbar_fence_init();
+  }
+  __syncthreads();
+  // Unit u of the group (K of tile u / 2, or V), by its whole first warp.
+  auto request = [&](int u) {
+    const int n = u >> 1, sl = u % D;
+    if (n >= mine) return;
+    if (n - pages_at >= 32) fetch_pages(n);
+    const int page = __shfl_sync(0xffffffffu, pages, n - pages_at);
+    if (lane != 0) return;
+    has[sl] = page >= 0;
+    if (page < 0) {
+      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&full[sl])) : "memory");
+      return;
+    }
+    const long long row = ((long long)page * p.kv_heads + kvh) * p.page_size + ((tile0 + tg + TG * n) % per_page) * 16;
+    uint8_t *to = ring + sl * S::UNIT;
+    mbar_expect_tx(&full[sl], 16 * S::ROW + (HALF && !(u & 1) ? 128 : 0));
+    bulk_g2s(to, (u & 1 ? p.v : p.k) + row * S::ROW, 16 * S::ROW, &full[sl]);
+    if (HALF && !(u & 1)) {
+      bulk_g2s(to + 16 * S::ROW, p.ks + row, 64, &full[sl]);
+      bulk_g2s(to + 16 * S::ROW + 64, p.vs + row, 64, &full[sl]);
+    }
+  };
+  if (rt == 0)
+    for (int u = 0; u < D; u++) request(u);
+
   uint2 *qs = reinterpret_cast<uint2 *>(dsm);   // [RT][NP][KSTEPS][32]
   __shared__ float q_scale[ROWS];
   __shared__ int row_lo[ROWS], row_hi[ROWS];
@@ -302,255 +360,219 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP>::OCC) k_
   for (int i = 0; i < HD / 16; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
 
-  // ---- this warp's tiles: tile0 + tg + TG n. Lane i holds the page of the i-th of 32 ahead.
-  const Pool &p = a.pool;
-  const int mine = tile1 - tile0 - tg > 0 ? (tile1 - tile0 - tg + TG - 1) / TG : 0;
-  const int per_page = p.page_size >> 4;
-  const int32_t *table = a.table + (long long)b * a.table_stride;
-  int pages = -1, pages_at = 0;
-  auto fetch_pages = [&](int n) {
-    const int k = n + lane;
-    pages = k < mine ? table[(tile0 + tg + TG * k) / per_page] : -1;
-    if (k < mine && (pages < 0 || pages >= p.n_pages)) {
-      paged_raise(a.err, G4_PAGED_BAD_PAGE);
-      pages = -1;
+  bool bad = false;   // a wait gave up: go on without waiting (the call is reported as not complete)
+  auto wait = [&](uint64_t *bar, uint32_t parity) {
+    if (!bad && !mbar_wait(bar, parity)) bad = true;
+  };
+  // This warp is done with unit u; the first warp of the group asks for the unit that takes its place.
+  auto release = [&](int u) {
+    __syncwarp();
+    if (RT > 1) {
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&empty[u % D])) : "memory");
+      if (rt == 0 && (u + D) >> 1 < mine) wait(&empty[u % D], (uint32_t)((u / D) & 1));
+      __syncwarp();
     }
-    pages_at = n;
+    if (rt == 0) request(u + D);
   };
-  // Position row (in rows of the pool) of the n-th tile's first position; -1 where its page is none.
-  auto tile_row = [&](int n) -> long long {
-    const int page = __shfl_sync(0xffffffffu, pages, (n - pages_at) & 31);
-    const int tile = tile0 + tg + TG * n;
-    return page < 0 ? -1 : ((long long)page * p.kv_heads + kvh) * p.page_size + (tile % per_page) * 16;
-  };
+  auto lds16 = [](const uint8_t *at) { return *reinterpret_cast<const uint4 *>(at); };
 
-  uint4 buf[S::NB][4];
-  // Chunk q of the tile whose first row is `row`: K chunks first, then V.
-  auto load_chunk = [&](uint4 (&d)[4], int q, long long row) {
-    if (row < 0) {
-#pragma unroll
-      for (int i = 0; i < 4; i++) d[i] = make_uint4(0, 0, 0, 0);
-      return;
-    }
-    auto ld16 = [&](const uint8_t *at) { return RT == 1 ? ldg_stream(at) : __ldg(reinterpret_cast<const uint4 *>(at)); };
-    if (q < S::HC) {
-      const uint8_t *k = p.k + row * S::ROW + g * S::ROW + c * 16 + q * 128;
-      d[0] = ld16(k);
-      d[1] = ld16(k + 8 * S::ROW);
-      if (!S::NARROW) {
-        d[2] = ld16(k + 64);
-        d[3] = ld16(k + 64 + 8 * S::ROW);
+#pragma unroll 1
+  for (int n = 0; n < mine; n++) {
+    const int uk = 2 * n, uv = 2 * n + 1;
+    const int pos0 = (tile0 + tg + TG * n) * 16;
+    wait(&full[uk % D], (uint32_t)((uk / D) & 1));
+    const bool on = has[uk % D];
+    float sa[4] = {0, 0, 0, 0}, sb[4] = {0, 0, 0, 0};
+    float ks0 = 1.0f, ks1 = 1.0f, w0 = 1.0f, w1 = 1.0f;
+    const uint8_t *unit = ring + (uk % D) * S::UNIT;
+    if (on) {
+      const uint8_t *kp = unit + g * S::ROW + c * 16;
+      if (HALF) {
+        const float *f = reinterpret_cast<const float *>(unit + 16 * S::ROW);
+        ks0 = f[g];
+        ks1 = f[g + 8];
+        w0 = f[16 + g];
+        w1 = f[24 + g];
       }
-    } else {
-      const uint8_t *v = p.v + row * S::ROW + 2 * c * S::ROW + (S::NARROW ? g * 8 : g * 16 + (q - S::HC) * 128);
+      constexpr int ST = HALF ? 4 : 2;
+#pragma unroll 2
+      for (int m = 0; m < S::ROW / 64; m++) {
+        const uint4 x = lds16(kp + 64 * m), y = lds16(kp + 64 * m + 8 * S::ROW);
+        const uint32_t r0[4] = {x.x, x.y, x.z, x.w}, r1[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const uint8_t *at = v + ((i & 1) + (i >> 1) * 8) * S::ROW;
-        if (S::NARROW) {
-          const uint2 w = __ldg(reinterpret_cast<const uint2 *>(at));
-          d[i] = make_uint4(w.x, w.y, 0, 0);
-        } else {
-          d[i] = ld16(at);
-        }
-      }
-    }
-  };
-  // Scales of positions g and g + 8 of the tile.
-  float ks0 = 1.0f, ks1 = 1.0f, vs0 = 1.0f, vs1 = 1.0f;
-  auto load_scales = [&](long long row) {
-    if (HALF && row >= 0) {
-      ks0 = __ldg(p.ks + row + g);
-      ks1 = __ldg(p.ks + row + g + 8);
-      vs0 = __ldg(p.vs + row + g);
-      vs1 = __ldg(p.vs + row + g + 8);
-    }
-  };
-
-  // Rows of the tiles the ring reaches into: [0] the one at hand.
-  long long rows_[S::TILES + 2];
-  if (mine > 0) fetch_pages(0);
-#pragma unroll
-  for (int i = 0; i < S::TILES + 2; i++) rows_[i] = i < mine ? tile_row(i) : -1;
-  load_scales(rows_[0]);
-#pragma unroll
-  for (int q = 0; q < S::NB - 1; q++) load_chunk(buf[q], q % S::C, rows_[q / S::C]);
-
-  for (int n0 = 0; n0 < mine; n0 += S::TILES) {
-#pragma unroll
-    for (int u = 0; u < S::TILES; u++) {
-      const int n = n0 + u;
-      const bool on = n < mine && rows_[u] >= 0;   // the same for the whole warp
-      const int pos0 = (tile0 + tg + TG * n) * 16;
-      float sa[4] = {0, 0, 0, 0}, sb[4] = {0, 0, 0, 0};
-      uint32_t pw[2][NP];
-      uint32_t dead = 0;
-#pragma unroll
-      for (int q = 0; q < S::C; q++) {
-        const int at = u * S::C + q;
-        {
-          const int ahead = at + S::NB - 1;
-          load_chunk(buf[ahead % S::NB], ahead % S::C, rows_[ahead / S::C]);
-        }
-        const uint4 (&w)[4] = buf[at % S::NB];
-        if (q < S::HC) {
-#pragma unroll
-          for (int h = 0; h < (S::NARROW ? 1 : 2); h++) {
-            const uint32_t r0[4] = {w[2 * h].x, w[2 * h].y, w[2 * h].z, w[2 * h].w};
-            const uint32_t r1[4] = {w[2 * h + 1].x, w[2 * h + 1].y, w[2 * h + 1].z, w[2 * h + 1].w};
-            constexpr int ST = HALF ? 4 : 2;
-#pragma unroll
-            for (int j = 0; j < ST; j++) {
-              uint32_t a0, a1, a2, a3;
-              if constexpr (HALF) {
-                codes4<FMT>(r0[j], a0, a2);
-                codes4<FMT>(r1[j], a1, a3);
-              } else {
-                a0 = r0[2 * j];
-                a2 = r0[2 * j + 1];
-                a1 = r1[2 * j];
-                a3 = r1[2 * j + 1];
-              }
-              const int step = (q * 2 + h) * ST + j;
-#pragma unroll
-              for (int k = 0; k < NP; k++) {
-                const uint2 bq = qw[(k * S::KSTEPS + step) * 32];
-                if (step & 1)
-                  mma16816<HALF>(sb, a0, a1, a2, a3, bq.x, bq.y);
-                else
-                  mma16816<HALF>(sa, a0, a1, a2, a3, bq.x, bq.y);
-              }
-            }
+        for (int j = 0; j < ST; j++) {
+          uint32_t a0, a1, a2, a3;
+          if constexpr (HALF) {
+            codes4<FMT>(r0[j], a0, a2);
+            codes4<FMT>(r1[j], a1, a3);
+          } else {
+            a0 = r0[2 * j];
+            a2 = r0[2 * j + 1];
+            a1 = r1[2 * j];
+            a3 = r1[2 * j + 1];
           }
-        }
-        if (q == S::HC - 1) {
-          // ---- softmax of the tile: sa[0], sa[1] are position g of rows 2c, 2c + 1; sa[2], sa[3] g + 8.
-          float s0 = (sa[0] + sb[0]) * (ks0 * qf0), s1 = (sa[1] + sb[1]) * (ks0 * qf1);
-          float s2 = (sa[2] + sb[2]) * (ks1 * qf0), s3 = (sa[3] + sb[3]) * (ks1 * qf1);
-          float w0 = vs0, w1 = vs1;
-          bool see0 = on, see1 = on, see2 = on, see3 = on;
-          const bool whole = on && pos0 >= all_lo && pos0 + 16 <= all_hi;
-          if (!whole && on) {
-            const int t0 = pos0 + g, t1 = t0 + 8;
-            see0 = t0 >= lo0 && t0 < hi0;
-            see1 = t0 >= lo1 && t0 < hi1;
-            see2 = t1 >= lo0 && t1 < hi0;
-            see3 = t1 >= lo1 && t1 < hi1;
-            // Positions whose V must not enter the product: those outside every row's range, and
-            // in bf16 pages those that hold an infinity or a NaN (0 times it is NaN for a row
-            // that does not see it); the rows that do see one get a NaN weight.
-            const unsigned live0 = __ballot_sync(0xffffffffu, see0 || see1), live1 = __ballot_sync(0xffffffffu, see2 || see3);
-            uint32_t live = 0;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-              if ((live0 >> (4 * i)) & 0xf) live |= 1u << i;
-              if ((live1 >> (4 * i)) & 0xf) live |= 1u << (i + 8);
-            }
-            dead = ~live & 0xffffu;
-            if constexpr (!HALF) {
-              uint32_t bad = 0;
-              for (int i = 0; i < 16; i++) {
-                const uint8_t *v = p.v + (rows_[u] + i) * S::ROW;
-                bool x = false;
-                for (int d = lane; d < HD / 2; d += 32) {
-                  const uint32_t z = *reinterpret_cast<const uint32_t *>(v + 4 * d);
-                  x |= (z & 0x7f80u) == 0x7f80u || (z & 0x7f800000u) == 0x7f800000u;
-                }
-                if (__any_sync(0xffffffffu, x)) bad |= 1u << i;
-              }
-              dead |= bad;
-              if ((bad >> g) & 1) w0 = __int_as_float(0x7fffffff);
-              if ((bad >> (g + 8)) & 1) w1 = __int_as_float(0x7fffffff);
-            }
-          }
-          const float g0 = HALF ? __log2f(fmaxf(w0, 0x1p-100f)) : 0.0f, g1 = HALF ? __log2f(fmaxf(w1, 0x1p-100f)) : 0.0f;
-          s0 = see0 ? s0 : -INFINITY;
-          s1 = see1 ? s1 : -INFINITY;
-          s2 = see2 ? s2 : -INFINITY;
-          s3 = see3 ? s3 : -INFINITY;
-          float n0_ = fmaxf(s0 + g0, s2 + g1), n1_ = fmaxf(s1 + g0, s3 + g1);
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) {
-            n0_ = fmaxf(n0_, __shfl_xor_sync(0xffffffffu, n0_, x));
-            n1_ = fmaxf(n1_, __shfl_xor_sync(0xffffffffu, n1_, x));
-          }
-          n0_ = fmaxf(n0_, m0);
-          n1_ = fmaxf(n1_, m1);
-          if (__any_sync(0xffffffffu, n0_ > m0 || n1_ > m1)) {
-            const float f0 = n0_ > m0 ? ex2(m0 - n0_) : 1.0f, f1 = n1_ > m1 ? ex2(m1 - n1_) : 1.0f;
-            l0 = n0_ > m0 ? rescale(l0, m0 - n0_) : l0;
-            l1 = n1_ > m1 ? rescale(l1, m1 - n1_) : l1;
-#pragma unroll
-            for (int i = 0; i < HD / 16; i++) {
-              o[i][0] *= f0;
-              o[i][1] *= f1;
-              o[i][2] *= f0;
-              o[i][3] *= f1;
-            }
-            m0 = n0_;
-            m1 = n1_;
-          }
-          const float bits = HALF ? kWeightBits : 0.0f;
-          const float r0 = m0 == -INFINITY ? 0.0f : m0 - bits, r1 = m1 == -INFINITY ? 0.0f : m1 - bits;
-          const float p0 = ex2(s0 - r0), p1 = ex2(s1 - r1), p2 = ex2(s2 - r0), p3 = ex2(s3 - r1);
-          l0 += p0 + p2;
-          l1 += p1 + p3;
-          uint32_t x[NP], y[NP];
-          split2<HALF, NP>(see0 ? p0 * w0 : 0.0f, see1 ? p1 * w0 : 0.0f, x);
-          split2<HALF, NP>(see2 ? p2 * w1 : 0.0f, see3 ? p3 * w1 : 0.0f, y);
 #pragma unroll
           for (int k = 0; k < NP; k++) {
-            pw[0][k] = transpose8x8(x[k]);
-            pw[1][k] = transpose8x8(y[k]);
-          }
-          load_scales(u + 1 < S::TILES ? rows_[u + 1] : rows_[S::TILES]);
-        }
-        if (q >= S::HC) {
-          uint4 v[4] = {w[0], w[1], w[2], w[3]};
-          if (dead) {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-              if ((dead >> (2 * c + (i & 1) + (i >> 1) * 8)) & 1) v[i] = make_uint4(0, 0, 0, 0);
-          }
-          const uint32_t vw[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
-                                     {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
-          constexpr int WORDS = S::NARROW ? 2 : 4;
-          const int ob = (q - S::HC) * (HALF ? 8 : 4);
-#pragma unroll
-          for (int j = 0; j < WORDS; j++) {
-            if constexpr (HALF) {
-              // Four dimensions of the pairs (2c, 2c + 1) and (2c + 8, 2c + 9).
-              uint32_t e[2][4];
-#pragma unroll
-              for (int h = 0; h < 2; h++) {
-                const uint32_t t0 = __byte_perm(vw[2 * h][j], vw[2 * h + 1][j], 0x5140);
-                const uint32_t t1 = __byte_perm(vw[2 * h][j], vw[2 * h + 1][j], 0x7362);
-                codes4<FMT>(t0, e[h][0], e[h][1]);
-                codes4<FMT>(t1, e[h][2], e[h][3]);
-              }
-#pragma unroll
-              for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int k = 0; k < NP; k++)
-                  mma16816<HALF>(o[ob + 2 * j + i], e[0][2 * i], e[0][2 * i + 1], e[1][2 * i], e[1][2 * i + 1], pw[0][k], pw[1][k]);
-            } else {
-              const uint32_t a0 = __byte_perm(vw[0][j], vw[1][j], 0x5410), a1 = __byte_perm(vw[0][j], vw[1][j], 0x7632);
-              const uint32_t a2 = __byte_perm(vw[2][j], vw[3][j], 0x5410), a3 = __byte_perm(vw[2][j], vw[3][j], 0x7632);
-#pragma unroll
-              for (int k = 0; k < NP; k++) mma16816<HALF>(o[ob + j], a0, a1, a2, a3, pw[0][k], pw[1][k]);
-            }
+            const uint2 bq = qw[(k * S::KSTEPS + m * ST + j) * 32];
+            if (j & 1)
+              mma16816<HALF>(sb, a0, a1, a2, a3, bq.x, bq.y);
+            else
+              mma16816<HALF>(sa, a0, a1, a2, a3, bq.x, bq.y);
           }
         }
       }
     }
-    // The next pass's tiles.
-    if (n0 + S::TILES < mine) {
-      const int base = n0 + S::TILES;
+    release(uk);
+    // ---- softmax of the tile: sa[0], sa[1] are position g of rows 2c, 2c + 1; sa[2], sa[3] g + 8.
+    float s0 = (sa[0] + sb[0]) * (ks0 * qf0), s1 = (sa[1] + sb[1]) * (ks0 * qf1);
+    float s2 = (sa[2] + sb[2]) * (ks1 * qf0), s3 = (sa[3] + sb[3]) * (ks1 * qf1);
+    bool see0 = on, see1 = on, see2 = on, see3 = on;
+    const bool whole = on && pos0 >= all_lo && pos0 + 16 <= all_hi;
+    uint32_t dead = 0;   // positions that no row of the warp sees
+    if (!whole && on) {
+      const int t0 = pos0 + g, t1 = t0 + 8;
+      see0 = t0 >= lo0 && t0 < hi0;
+      see1 = t0 >= lo1 && t0 < hi1;
+      see2 = t1 >= lo0 && t1 < hi0;
+      see3 = t1 >= lo1 && t1 < hi1;
+      const unsigned live0 = __ballot_sync(0xffffffffu, see0 || see1), live1 = __ballot_sync(0xffffffffu, see2 || see3);
 #pragma unroll
-      for (int i = 0; i < 2; i++) rows_[i] = rows_[S::TILES + i];
-      if (base + S::TILES + 1 - pages_at >= 32) fetch_pages(base);
-#pragma unroll
-      for (int i = 2; i < S::TILES + 2; i++) rows_[i] = base + i < mine ? tile_row(base + i) : -1;
+      for (int i = 0; i < 8; i++) {
+        if (!((live0 >> (4 * i)) & 0xf)) dead |= 1u << i;
+        if (!((live1 >> (4 * i)) & 0xf)) dead |= 1u << (i + 8);
+      }
     }
+    const float g0 = HALF ? __log2f(fmaxf(w0, 0x1p-100f)) : 0.0f, g1 = HALF ? __log2f(fmaxf(w1, 0x1p-100f)) : 0.0f;
+    s0 = see0 ? s0 : -INFINITY;
+    s1 = see1 ? s1 : -INFINITY;
+    s2 = see2 ? s2 : -INFINITY;
+    s3 = see3 ? s3 : -INFINITY;
+    float n0 = fmaxf(s0 + g0, s2 + g1), n1 = fmaxf(s1 + g0, s3 + g1);
+#pragma unroll
+    for (int x = 4; x < 32; x <<= 1) {
+      n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
+      n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
+    }
+    n0 = fmaxf(n0, m0);
+    n1 = fmaxf(n1, m1);
+    if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
+      const float f0 = n0 > m0 ? ex2(m0 - n0) : 1.0f, f1 = n1 > m1 ? ex2(m1 - n1) : 1.0f;
+      l0 = n0 > m0 ? rescale(l0, m0 - n0) : l0;
+      l1 = n1 > m1 ? rescale(l1, m1 - n1) : l1;
+#pragma unroll
+      for (int i = 0; i < HD / 16; i++) {
+        o[i][0] *= f0;
+        o[i][1] *= f1;
+        o[i][2] *= f0;
+        o[i][3] *= f1;
+      }
+      m0 = n0;
+      m1 = n1;
+    }
+    uint32_t pw[2][NP];
+    {
+      const float bits = HALF ? kWeightBits : 0.0f;
+      const float r0 = m0 == -INFINITY ? 0.0f : m0 - bits, r1 = m1 == -INFINITY ? 0.0f : m1 - bits;
+      const float p0 = ex2(s0 - r0), p1 = ex2(s1 - r1), p2 = ex2(s2 - r0), p3 = ex2(s3 - r1);
+      l0 += p0 + p2;
+      l1 += p1 + p3;
+      uint32_t x[NP], y[NP];
+      split2<HALF, NP>(see0 ? p0 * w0 : 0.0f, see1 ? p1 * w0 : 0.0f, x);
+      split2<HALF, NP>(see2 ? p2 * w1 : 0.0f, see3 ? p3 * w1 : 0.0f, y);
+#pragma unroll
+      for (int k = 0; k < NP; k++) {
+        pw[0][k] = transpose8x8(x[k]);
+        pw[1][k] = transpose8x8(y[k]);
+      }
+    }
+    wait(&full[uv % D], (uint32_t)((uv / D) & 1));
+    if (on) {
+      const uint8_t *vp = ring + (uv % D) * S::UNIT + 2 * c * S::ROW + g * (S::NARROW ? 8 : 16);
+      uint32_t odd = 0;   // bf16 pages: this lane met a value that is not finite at its i-th position
+      constexpr int MM = S::NARROW ? 1 : S::ROW / 128;
+#pragma unroll
+      for (int mm = 0; mm < MM; mm++) {
+        uint4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const uint8_t *at = vp + ((i & 1) + (i >> 1) * 8) * S::ROW + mm * 128;
+          if (S::NARROW) {
+            const uint2 w = *reinterpret_cast<const uint2 *>(at);
+            v[i] = make_uint4(w.x, w.y, 0, 0);
+          } else {
+            v[i] = lds16(at);
+          }
+        }
+        if (FMT != G4_PAGE_INT8 && !whole) {
+          // What no row sees may be anything, and 0 times an infinity or a NaN is NaN. e4m3 codes of
+          // stored rows are finite; in bf16 pages a row may see a position that another does not.
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            if ((dead >> (2 * c + (i & 1) + (i >> 1) * 8)) & 1) v[i] = make_uint4(0, 0, 0, 0);
+            if constexpr (!HALF) {
+              uint32_t z[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+              for (int k = 0; k < 4; k++) {
+                if ((z[k] & 0x7f80u) == 0x7f80u) {
+                  z[k] &= 0xffff0000u;
+                  odd |= 1u << i;
+                }
+                if ((z[k] & 0x7f800000u) == 0x7f800000u) {
+                  z[k] &= 0xffffu;
+                  odd |= 1u << i;
+                }
+              }
+              v[i] = make_uint4(z[0], z[1], z[2], z[3]);
+            }
+          }
+        }
+        const uint32_t vw[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
+                                   {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
+        constexpr int WORDS = S::NARROW ? 2 : 4;
+        const int ob = mm * (HALF ? 8 : 4);
+#pragma unroll
+        for (int j = 0; j < WORDS; j++) {
+          if constexpr (HALF) {
+            // Four dimensions of the pairs (2c, 2c + 1) and (2c + 8, 2c + 9).
+            uint32_t e[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              const uint32_t t0 = __byte_perm(vw[2 * h][j], vw[2 * h + 1][j], 0x5140);
+              const uint32_t t1 = __byte_perm(vw[2 * h][j], vw[2 * h + 1][j], 0x7362);
+              codes4<FMT>(t0, e[h][0], e[h][1]);
+              codes4<FMT>(t1, e[h][2], e[h][3]);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+              for (int k = 0; k < NP; k++)
+                mma16816<HALF>(o[ob + 2 * j + i], e[0][2 * i], e[0][2 * i + 1], e[1][2 * i], e[1][2 * i + 1], pw[0][k], pw[1][k]);
+          } else {
+            const uint32_t a0 = __byte_perm(vw[0][j], vw[1][j], 0x5410), a1 = __byte_perm(vw[0][j], vw[1][j], 0x7632);
+            const uint32_t a2 = __byte_perm(vw[2][j], vw[3][j], 0x5410), a3 = __byte_perm(vw[2][j], vw[3][j], 0x7632);
+#pragma unroll
+            for (int k = 0; k < NP; k++) mma16816<HALF>(o[ob + j], a0, a1, a2, a3, pw[0][k], pw[1][k]);
+          }
+        }
+      }
+      if (!HALF && __any_sync(0xffffffffu, odd != 0)) {
+        // Rows that see such a position are not finite.
+        uint32_t lanes[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) lanes[i] = __ballot_sync(0xffffffffu, (odd >> i) & 1);
+        const uint32_t of = 0x11111111u << (g >> 1);
+        const bool b0 = ((g & 1) ? lanes[1] : lanes[0]) & of, b1 = ((g & 1) ? lanes[3] : lanes[2]) & of;
+        const float nan = __int_as_float(0x7fffffff);
+        if ((b0 && see0) || (b1 && see2)) l0 = nan;
+        if ((b0 && see1) || (b1 && see3)) l1 = nan;
+      }
+    }
+    release(uv);
+  }
+  if (bad) {
+    paged_raise(a.err, G4_PAGED_TIMEOUT);
+    // What was asked for has landed, or a second limit has passed, before the ring is given up.
+    for (int u = 2 * mine > D ? 2 * mine - D : 0; u < 2 * mine; u++) mbar_wait(&full[u % D], (uint32_t)((u / D) & 1));
   }
 
   // ---- join the token groups through shared memory (over Q), then write out or leave a partial.
@@ -565,7 +587,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP>::OCC) k_
   float *sm = reinterpret_cast<float *>(dsm) + tg * PART;
 #pragma unroll
   for (int q = 0; q < HD / 16; q++) {
-    // Accumulator q: the chunk's dimensions 16 g + 2 j (8 bit; 8 g + 2 j narrow or at 16 bits) and the next.
+    // Accumulator q: dimensions 16 g + 2 j of a 128-byte column (8 bit; 8 g + 2 j narrow or at 16 bits) and the next.
     constexpr int PER = S::NARROW ? 4 : (HALF ? 8 : 4);
     const int chunk = q / PER, j = q % PER;
     const int d = chunk * (HALF && !S::NARROW ? 128 : 64) + g * (HALF && !S::NARROW ? 16 : 8) + 2 * j;
@@ -690,7 +712,7 @@ static void plan_decode(PagedAttn &a) {
   }
   const int tiles = (int)((span + 15) / 16) > 0 ? (int)((span + 15) / 16) : 1;
   const long long base = (long long)a.batch * a.pool.kv_heads * a.row_groups;
-  const int occ = a.pool.hd <= 256 ? 3 : 2;
+  const int occ = 2;
   long long want = (2ll * 148 * occ + base - 1) / base;
   const long long most = (tiles + tg - 1) / tg;
   if (want > most) want = most;
@@ -712,9 +734,8 @@ size_t paged_attention_partials(const PagedAttn &args) {
 
 template <int FMT, int HD, int NP, int RT>
 static cudaError_t launch_decode_rt(const PagedAttn &a, cudaStream_t st) {
-  using S = DecShape<FMT, HD, NP>;
-  constexpr int QB = RT * NP * S::KSTEPS * 32 * 8, OB = kDecWarps / RT * 8 * RT * (HD + 2) * 4;
-  constexpr int SMEM = QB > OB ? QB : OB;
+  using S = DecShape<FMT, HD, NP, RT>;
+  constexpr int SMEM = S::SMEM;
   static DeviceOnce once;
   cudaError_t e = cudaSuccess;
   once([&] { e = cudaFuncSetAttribute(k_paged_decode<FMT, HD, NP, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); });

@@ -28,10 +28,9 @@ struct PagedAttn {
   const int32_t *q_begin, *q_pos, *kv_len, *table;
   int table_stride, max_q, max_kv, window;
   float scale;
-  // The split over the context (set by the launcher): tiles of 16 positions per split, splits per
-  // sequence, row groups per (sequence, KV head); the splits' partials and the counts of finished
-  // ones.
-  int split_tiles, splits, row_groups;
+  // Set by the launcher: the least tiles of 16 positions a block takes, the row groups per (sequence,
+  // KV head); the blocks' partials and the counts of finished ones.
+  int split_tiles, row_groups;
   float *part;
   uint32_t *count;
   int *err;
@@ -77,7 +76,7 @@ __device__ __forceinline__ void paged_raise(int *flags, int bit) { atomicOr(flag
 struct SeqSpan {
   int row, n, pos, kv;
 };
-__device__ __forceinline__ SeqSpan seq_span(const PagedAttn &a, int b) {
+__device__ __forceinline__ SeqSpan seq_span(const PagedAttn &a, int b, bool report = true) {
   const int b0 = a.q_begin[b], b1 = a.q_begin[b + 1], kv = a.kv_len[b], pos = a.q_pos[b];
   SeqSpan s;
   s.row = min(max(b0, 0), a.rows);
@@ -86,7 +85,7 @@ __device__ __forceinline__ SeqSpan seq_span(const PagedAttn &a, int b) {
   s.kv = min(max(kv, 0), a.max_kv);
   // Positions lie in 0 .. 2^30, so sums with a row index stay in 32 bits.
   s.pos = min(max(pos, -(1 << 30)), 1 << 30);
-  if (b0 < 0 || b1 < b0 || b1 > a.rows || end - s.row > a.max_q || kv < 0 || kv > a.max_kv || s.pos != pos)
+  if (report && (b0 < 0 || b1 < b0 || b1 > a.rows || end - s.row > a.max_q || kv < 0 || kv > a.max_kv || s.pos != pos))
     paged_raise(a.err, G4_PAGED_BAD_LENGTH);
   return s;
 }

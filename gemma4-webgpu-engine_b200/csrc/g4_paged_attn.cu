@@ -19,12 +19,17 @@
 //    8 x 8 transpose in registers turns S^T's layout into P^T's.
 //  - f32 rows: q and p vs are carried in two f16 parts (8-bit codes; 22 bits together) or three
 //    bf16 parts (bf16 pages), one product each, all accumulated in f32.
-// The warp groups of a block take a split's tiles in turn and join through shared memory. A context that
-// one block per (sequence, KV head) would leave most SMs idle for is split over blocks; the
-// last of 16 splits to finish joins them, and the last such group joins the groups (one block
-// would read 2.4 MB alone for 148 splits of head_dim 512).
+// The work is one list: every (sequence, KV head, 8 RT rows) with its tiles, end to end. Each of a fixed
+// number of blocks, as many as the SMs hold at once, takes an equal share of the list, so ragged
+// lengths cost nothing (64 contexts of 128 .. 4,096 positions at head_dim 512: 68 us with a grid of
+// equal splits, of which half the slots were empty and the rest worked in two rounds). A block's
+// share may begin or end inside a context; such parts are joined by the last of 16 neighbours to
+// finish, and those by the last of them (one block would read 2.4 MB alone for 148 parts of
+// head_dim 512).
 #include <cuda_runtime.h>
 #include <math.h>
+
+#include <algorithm>
 
 #include "g4_device.cuh"
 #include "g4_kernels.cuh"
@@ -109,6 +114,9 @@ __device__ __forceinline__ void split2(float v0, float v1, uint32_t (&out)[NP]) 
   }
 }
 
+// Blocks an SM holds by registers.
+constexpr int most_blocks(int hd) { return hd == 512 ? 2 : (hd == 256 ? 3 : 4); }
+
 template <int FMT, int HD, int NP, int RT>
 struct DecShape {
   static constexpr bool HALF = FMT != G4_PAGE_BF16;
@@ -119,30 +127,34 @@ struct DecShape {
   static constexpr int TG = kDecWarps / RT;            // groups of warps, a ring each
   static constexpr int UNIT = 16 * ROW + (HALF ? 128 : 0);   // K's (with both scales) or V's 16 positions
   static constexpr int Q_BYTES = RT * NP * KSTEPS * 32 * 8;
-  // Two blocks on an SM where three units a ring fit into half of its shared memory.
-  static constexpr int D2 = (108 * 1024 - Q_BYTES) / (TG * UNIT), D1 = (222 * 1024 - Q_BYTES) / (TG * UNIT);
-  static constexpr int OCC = D2 >= 3 ? 2 : 1;
-  static constexpr int DD = OCC == 2 ? D2 : D1, D = DD > 8 ? 8 : DD;
+  // Blocks on an SM: as many as the registers allow (O takes HD / 4 of them) with three units a ring.
+  static constexpr int ring_depth(int occ) { return ((occ == 1 ? 220 : 216 / occ) * 1024 - 1024 * 4 - Q_BYTES) / (TG * UNIT); }
+  static constexpr int MOST = most_blocks(HD);
+  static constexpr int OCC = ring_depth(MOST) >= 3 ? MOST : (ring_depth(2) >= 3 ? 2 : 1);
+  static constexpr int DD = ring_depth(OCC), D = DD > 8 ? 8 : DD;
   static_assert(D >= 2, "a ring holds K and V of a tile");
   static constexpr int RING = TG * D * UNIT, JOIN = TG * 8 * RT * (HD + 2) * 4;
   static constexpr int SMEM = Q_BYTES + RING > JOIN ? Q_BYTES + RING : JOIN;
 };
 
-// The join of `np` partials of `rows` rows (o [rows][HD], then m [rows], l [rows] each `stride`
-// floats apart): every thread takes part; result rows go to out/lse or to another partial.
+// The join of `np` partials of `rows` rows (o [rows][HD], then m [rows], l [rows]), the first at `first`,
+// the others `stride` floats apart from `rest` on: every thread takes part; result rows go to out and
+// lse, or to another partial (`to`, which may be the first: each thread reads an element of all before
+// it writes it).
 template <int HD>
-__device__ __forceinline__ void join_partials(const PagedAttn &a, const float *parts, long long stride, int np, int rows,
+__device__ __forceinline__ void join_partials(const PagedAttn &a, const float *first, const float *rest, long long stride, int np, int rows,
                                               float *to, const SeqSpan &s, int kvh, int row0, float bits, float *fsh) {
   // fsh: [np][rows] factors, then [rows] 1 / l.
   const int t = threadIdx.x, nt = blockDim.x;
+  auto part = [&](int i) { return i == 0 ? first : rest + (i - 1) * stride; };
   for (int r = t; r < rows; r += nt) {
     float M = -INFINITY;
-    for (int i = 0; i < np; i++) M = fmaxf(M, __ldcg(parts + i * stride + rows * HD + r));
+    for (int i = 0; i < np; i++) M = fmaxf(M, __ldcg(part(i) + rows * HD + r));
     float l = 0.0f;
     for (int i = 0; i < np; i++) {
-      const float m = __ldcg(parts + i * stride + rows * HD + r);
+      const float m = __ldcg(part(i) + rows * HD + r);
       fsh[i * rows + r] = M == -INFINITY ? 0.0f : ex2(m - M);
-      l += rescale(__ldcg(parts + i * stride + rows * HD + rows + r), M == -INFINITY ? 0.0f : m - M);
+      l += rescale(__ldcg(part(i) + rows * HD + rows + r), M == -INFINITY ? 0.0f : m - M);
     }
     fsh[np * rows + r] = l;
     const int rr = row0 + r, i = rr / a.group;
@@ -162,7 +174,7 @@ __device__ __forceinline__ void join_partials(const PagedAttn &a, const float *p
 #pragma unroll 8
     for (int k = 0; k < np; k++) {
       const float f = fsh[k * rows + r];
-      const float4 v = __ldcg(reinterpret_cast<const float4 *>(parts + k * stride + r * HD + d));
+      const float4 v = __ldcg(reinterpret_cast<const float4 *>(part(k) + r * HD + d));
       o.x = fmaf(f, v.x, o.x);
       o.y = fmaf(f, v.y, o.y);
       o.z = fmaf(f, v.z, o.z);
@@ -184,31 +196,141 @@ __device__ __forceinline__ void join_partials(const PagedAttn &a, const float *p
   }
 }
 
-// Block (row group x KV head, split, sequence): 8 RT rows; RT warps share each tile of positions,
-// one row tile of 8 each, and 4 / RT tiles are worked on side by side.
+// RT warps share each tile of positions, one row tile of 8 each; 4 / RT tiles are worked on side by side.
 template <int FMT, int HD, int NP, int RT>
 __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC) k_paged_decode(const PagedAttn a) {
   using S = DecShape<FMT, HD, NP, RT>;
   constexpr bool HALF = S::HALF;
-  constexpr int TG = S::TG, ROWS = 8 * RT, D = S::D;
+  constexpr int TG = S::TG, ROWS = 8 * RT, D = S::D, NT = kDecWarps * 32;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, g = lane >> 2, c = lane & 3;
   const int rt = warp % RT, tg = warp / RT;
-  const int split = blockIdx.y, rg = blockIdx.x % a.row_groups, kvh = blockIdx.x / a.row_groups, b = blockIdx.z;
-  const SeqSpan s = seq_span(a, b);
+  const Pool &p = a.pool;
+  const int per_page = p.page_size >> 4;
+
+  extern __shared__ __align__(128) uint8_t dsm[];   // Q, then the groups' rings; at the end the groups' partials
+  uint8_t *const ring = dsm + S::Q_BYTES + tg * D * S::UNIT;
+  __shared__ uint64_t full_[TG][D], empty_[TG][D];
+  __shared__ int has_[TG][D];   // whether the unit's page exists
+  __shared__ float q_scale[ROWS];
+  __shared__ int row_lo[ROWS], row_hi[ROWS];
+  __shared__ float fsh[(kJoin + 1) * ROWS];
+  __shared__ int sum_sh[kDecWarps + 4];
+  uint64_t *const full = full_[tg], *const empty = empty_[tg];
+  volatile int *const has = has_[tg];
+  if (t == 0) {
+    for (int i = 0; i < TG * D; i++) {
+      mbar_init(&full_[0][i], 1);
+      mbar_init(&empty_[0][i], RT);
+    }
+    mbar_fence_init();
+  }
+
+  // ---- the list. Tiles of row group rg of sequence s (one even where nothing is seen: zeros are
+  // written there), from its first.
+  auto tiles_of = [&](const SeqSpan &s, int rg, int &first) {
+    const int R = s.n * a.group, r0 = rg * ROWS;
+    if (r0 >= R) return 0;
+    int lo, hi, tmp;
+    row_range(a, s.pos + r0 / a.group, s.kv, lo, tmp);
+    row_range(a, s.pos + (min(r0 + ROWS, R) - 1) / a.group, s.kv, tmp, hi);
+    first = lo >> 4;
+    return hi > lo ? ((hi + 15) >> 4) - first : 1;
+  };
+  // All tiles of sequence b.
+  auto seq_tiles = [&](int b, bool report) -> long long {
+    const SeqSpan s = seq_span(a, b, report);
+    int n = 0, first;
+    for (int rg = 0; rg < a.row_groups; rg++) n += tiles_of(s, rg, first);
+    return (long long)n * p.kv_heads;
+  };
+  // Thread t holds the tiles of its share of the sequences; the block's scan gives where each begins.
+  const int per = (a.batch + NT - 1) / NT;
+  long long mine_sum = 0;
+  for (int i = 0; i < per; i++) {
+    const int b = t * per + i;
+    if (b < a.batch) mine_sum += seq_tiles(b, blockIdx.x == 0);
+  }
+  long long incl = mine_sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += o;
+  }
+  __shared__ long long warp_sum[kDecWarps];
+  if (lane == 31) warp_sum[warp] = incl;
+  __syncthreads();
+  long long before = incl - mine_sum, total = 0;
+#pragma unroll
+  for (int w = 0; w < kDecWarps; w++) {
+    if (w < warp) before += warp_sum[w];
+    total += warp_sum[w];
+  }
+  const long long share = max((total + gridDim.x - 1) / gridDim.x, (long long)a.split_tiles);
+  long long at = share * blockIdx.x;
+  const long long end = min(total, at + share);
+  if (at >= end) return;
+  // The sequence this block begins in, and where its tiles begin.
+  __shared__ long long seq_at_sh;
+  if (before <= at && at < before + mine_sum) {
+    long long x = before;
+    int b = t * per;
+    for (;; b++) {
+      const long long n = seq_tiles(b, false);
+      if (at < x + n) break;
+      x += n;
+    }
+    sum_sh[0] = b;
+    seq_at_sh = x;
+  }
+  __syncthreads();
+  int b = sum_sh[0];
+  long long seq_at = seq_at_sh;
+  int ubase = 0;   // units of the ring used by the parts before
+
+  bool bad = false;   // a wait gave up: go on without waiting (the call is reported as not complete)
+  auto wait = [&](uint64_t *bar, uint32_t parity) {
+    if (!bad && !mbar_wait(bar, parity)) bad = true;
+  };
+  auto lds16 = [](const uint8_t *at) { return *reinterpret_cast<const uint4 *>(at); };
+  uint2 *const qs = reinterpret_cast<uint2 *>(dsm);   // [RT][NP][KSTEPS][32]
+  const uint2 *const qw = qs + (size_t)rt * NP * S::KSTEPS * 32 + lane;
+
+#pragma unroll 1
+  while (at < end) {
+  // ---- the part at hand: KV head and row group of sequence b, its tiles tile0 .. tile1 - 1.
+  const SeqSpan s = seq_span(a, b, false);
+  int kvh = 0, rg = 0, first = 0, tiles;
+  long long item_at = seq_at;
+  {
+    int all = 0;
+    for (int r = 0; r < a.row_groups; r++) all += tiles_of(s, r, first);
+    if (at >= seq_at + (long long)all * p.kv_heads) {   // this sequence is done
+      seq_at += (long long)all * p.kv_heads;
+      b++;
+      continue;
+    }
+    kvh = (int)((at - seq_at) / all);
+    item_at += (long long)kvh * all;
+    tiles = tiles_of(s, 0, first);
+    while (at >= item_at + tiles) {
+      item_at += tiles;
+      tiles = tiles_of(s, ++rg, first);
+    }
+  }
   const int R = s.n * a.group, row0 = rg * ROWS;
-  if (row0 >= R) return;
-  int lo, hi, tmp;
-  row_range(a, s.pos + row0 / a.group, s.kv, lo, tmp);
-  row_range(a, s.pos + (min(row0 + ROWS, R) - 1) / a.group, s.kv, tmp, hi);
-  const int first = lo >> 4, last = hi > lo ? (hi + 15) >> 4 : first;
-  const int ns = max(1, (last - first + a.split_tiles - 1) / a.split_tiles);
-  if (split >= ns) return;
-  const int tile0 = first + split * a.split_tiles, tile1 = min(last, tile0 + a.split_tiles);
+  const int tile0 = first + (int)(at - item_at);
+  const int count = (int)min((long long)tiles - (at - item_at), end - at);
+  const bool complete = count == tiles;
+  int lo, hi;
+  {
+    int tmp;
+    row_range(a, s.pos + row0 / a.group, s.kv, lo, tmp);
+    row_range(a, s.pos + (min(row0 + ROWS, R) - 1) / a.group, s.kv, tmp, hi);
+  }
+  const int tile1 = hi > lo ? tile0 + count : tile0;   // (nothing seen: no tile to read)
 
   // ---- this group's tiles: tile0 + tg + TG n; its first warp asks for them.
-  const Pool &p = a.pool;
   const int mine = tile1 - tile0 - tg > 0 ? (tile1 - tile0 - tg + TG - 1) / TG : 0;
-  const int per_page = p.page_size >> 4;
   const int32_t *table = a.table + (long long)b * a.table_stride;
   // Lane i of the first warp holds the page of the i-th of 32 tiles from pages_at on (-1: none).
   int pages = -1, pages_at = 0;
@@ -223,23 +345,34 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
   };
   if (rt == 0 && mine > 0) fetch_pages(0);
 
-  extern __shared__ __align__(128) uint8_t dsm[];   // Q, then the groups' rings; at the end the groups' partials
-  uint8_t *ring = dsm + S::Q_BYTES + tg * D * S::UNIT;
-  __shared__ uint64_t full_[TG][D], empty_[TG][D];
-  __shared__ int has_[TG][D];   // whether the unit's page exists
-  uint64_t *full = full_[tg], *empty = empty_[tg];
-  volatile int *has = has_[tg];
-  if (t == 0) {
-    for (int i = 0; i < TG * D; i++) {
-      mbar_init(&full_[0][i], 1);
-      mbar_init(&empty_[0][i], RT);
+  // ---- Q: its loads go out before the first positions are asked for. One warp a row, two rows at a
+  // time; a lane takes four dimensions of each 128.
+  constexpr int QC = (HD + 127) / 128;
+  float4 qv[2][QC];
+  auto load_q = [&](int r, float4 (&v)[QC]) {
+    const int rr = row0 + r, i = rr / a.group;
+#pragma unroll
+    for (int j = 0; j < QC; j++) {
+      const int d = 128 * j + 4 * lane;
+      v[j] = make_float4(0, 0, 0, 0);
+      if (rr < R && d < HD) {
+        const long long from = (long long)(s.row + i) * a.q_stride + (long long)(kvh * a.group + rr % a.group) * HD + d;
+        if (a.type == G4_F32) {
+          v[j] = *reinterpret_cast<const float4 *>((const float *)a.q + from);
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2 *>((const __nv_bfloat16 *)a.q + from);
+          v[j] = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                             __uint_as_float(u.y & 0xffff0000u));
+        }
+      }
     }
-    mbar_fence_init();
-  }
-  __syncthreads();
+  };
+  load_q(warp, qv[0]);
+  load_q(warp + kDecWarps, qv[1]);
+
   // Unit u of the group (K of tile u / 2, or V), by its whole first warp.
   auto request = [&](int u) {
-    const int n = u >> 1, sl = u % D;
+    const int n = u >> 1, sl = (ubase + u) % D;
     if (n >= mine) return;
     if (n - pages_at >= 32) fetch_pages(n);
     const int page = __shfl_sync(0xffffffffu, pages, n - pages_at);
@@ -261,84 +394,50 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
   if (rt == 0)
     for (int u = 0; u < D; u++) request(u);
 
-  uint2 *qs = reinterpret_cast<uint2 *>(dsm);   // [RT][NP][KSTEPS][32]
-  __shared__ float q_scale[ROWS];
-  __shared__ int row_lo[ROWS], row_hi[ROWS];
-
-  // ---- Q into fragment order: for K step k of row tile r lane (g, c) holds four consecutive
-  // dimensions of row g. One warp a row.
-  for (int r = warp; r < ROWS; r += kDecWarps) {
-    const int rr = row0 + r, i = rr / a.group;
-    const bool on = rr < R;
-    float x[HD / 32];
-    // Lane l takes dimensions 4 l' .. + 3 of each 128.
-    float top = 0.0f;
+  // Q into fragment order: for K step k of row tile r lane (g, c) holds four consecutive dimensions of
+  // row g. 8-bit pages: f16 parts, scaled by a power of two that takes the row's greatest to 2^8 .. 2^9.
+#pragma unroll 1
+  for (int r0 = warp; r0 < ROWS; r0 += 2 * kDecWarps) {
+    if (r0 > warp) {
+      load_q(r0, qv[0]);
+      load_q(r0 + kDecWarps, qv[1]);
+    }
 #pragma unroll
-    for (int j = 0; j < (HD + 127) / 128; j++) {
-      const int d = 128 * j + 4 * lane;
-      float4 v = make_float4(0, 0, 0, 0);
-      if (on && d < HD) {
-        const long long at = (long long)(s.row + i) * a.q_stride + (long long)(kvh * a.group + rr % a.group) * HD + d;
-        if (a.type == G4_F32) {
-          v = *reinterpret_cast<const float4 *>((const float *)a.q + at);
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2 *>((const __nv_bfloat16 *)a.q + at);
-          v = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                          __uint_as_float(u.y & 0xffff0000u));
-        }
-      }
-      if constexpr (HD >= 128) {
-        x[4 * j] = v.x; x[4 * j + 1] = v.y; x[4 * j + 2] = v.z; x[4 * j + 3] = v.w;
-      }
-      top = fmaxf(fmaxf(fmaxf(top, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
-      if constexpr (HD < 128) {
-        x[0] = v.x; x[1] = v.y;   // lanes 0..15 hold four; the rest of them below
-      }
-      if constexpr (HD < 128) {
+    for (int z = 0; z < 2; z++) {
+      const int r = r0 + z * kDecWarps;
+      float top = 0.0f;
 #pragma unroll
-        for (int m = 1; m < 32; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-        int e = (int)((__float_as_uint(top) >> 23) & 0xff) - 127;
-        if (!HALF || e < -110 || e > 127) e = HALF && e < -110 ? -110 : 0;
-        const float f = HALF ? __uint_as_float((uint32_t)(127 + 8 - e) << 23) : 1.0f;
+      for (int j = 0; j < QC; j++)
+        top = fmaxf(fmaxf(fmaxf(top, fabsf(qv[z][j].x)), fmaxf(fabsf(qv[z][j].y), fabsf(qv[z][j].z))), fabsf(qv[z][j].w));
+      int e = 0;
+      if (HALF) {
+        // (Magnitudes order as their bits do.) Infinities and NaN stay what they are at any scale.
+        e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23) - 127;
+        e = e < -110 ? -110 : (e > 127 ? 0 : e);
+      }
+      const float f = HALF ? __uint_as_float((uint32_t)(127 + 8 - e) << 23) : 1.0f;
+#pragma unroll
+      for (int j = 0; j < QC; j++) {
+        const int d = 128 * j + 4 * lane;
         uint32_t p01[NP], p23[NP];
-        split2<HALF, NP>(v.x * f, v.y * f, p01);
-        split2<HALF, NP>(v.z * f, v.w * f, p23);
-        if (d < HD) {
-          // 8 bit: d = 64 m + 16 c + 4 j, step 4 m + j; 16 bit: d = 32 m + 8 c + 4 j, step 2 m + j.
-          const int step = HALF ? (d >> 6) * 4 + ((d >> 2) & 3) : (d >> 5) * 2 + ((d >> 2) & 1);
-          const int cc = HALF ? (d >> 4) & 3 : (d >> 3) & 3;
+        split2<HALF, NP>(qv[z][j].x * f, qv[z][j].y * f, p01);
+        split2<HALF, NP>(qv[z][j].z * f, qv[z][j].w * f, p23);
+        // 8 bit: d = 64 m + 16 c + 4 j, step 4 m + j; 16 bit: d = 32 m + 8 c + 4 j, step 2 m + j.
+        const int step = HALF ? (d >> 6) * 4 + ((d >> 2) & 3) : (d >> 5) * 2 + ((d >> 2) & 1);
+        const int cc = HALF ? (d >> 4) & 3 : (d >> 3) & 3;
+        if (d < HD && r < ROWS) {
 #pragma unroll
           for (int k = 0; k < NP; k++)
             qs[(((r >> 3) * NP + k) * S::KSTEPS + step) * 32 + (r & 7) * 4 + cc] = make_uint2(p01[k], p23[k]);
         }
-        if (lane == 0) q_scale[r] = a.scale * kLog2e * (HALF ? __uint_as_float((uint32_t)(127 - 8 + e) << 23) : 1.0f);
       }
-    }
-    if constexpr (HD >= 128) {
-#pragma unroll
-      for (int m = 1; m < 32; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-      int e = (int)((__float_as_uint(top) >> 23) & 0xff) - 127;
-      if (!HALF || e < -110 || e > 127) e = HALF && e < -110 ? -110 : 0;
-      const float f = HALF ? __uint_as_float((uint32_t)(127 + 8 - e) << 23) : 1.0f;
-#pragma unroll
-      for (int j = 0; j < HD / 128; j++) {
-        const int d = 128 * j + 4 * lane;
-        uint32_t p01[NP], p23[NP];
-        split2<HALF, NP>(x[4 * j] * f, x[4 * j + 1] * f, p01);
-        split2<HALF, NP>(x[4 * j + 2] * f, x[4 * j + 3] * f, p23);
-        const int step = HALF ? (d >> 6) * 4 + ((d >> 2) & 3) : (d >> 5) * 2 + ((d >> 2) & 1);
-        const int cc = HALF ? (d >> 4) & 3 : (d >> 3) & 3;
-#pragma unroll
-        for (int k = 0; k < NP; k++)
-          qs[(((r >> 3) * NP + k) * S::KSTEPS + step) * 32 + (r & 7) * 4 + cc] = make_uint2(p01[k], p23[k]);
+      if (lane == 0 && r < ROWS) {
+        q_scale[r] = a.scale * kLog2e * (HALF ? __uint_as_float((uint32_t)(127 - 8 + e) << 23) : 1.0f);
+        int x0 = 0, x1 = 0;
+        if (row0 + r < R) row_range(a, s.pos + (row0 + r) / a.group, s.kv, x0, x1);
+        row_lo[r] = x0;
+        row_hi[r] = x1;
       }
-      if (lane == 0) q_scale[r] = a.scale * kLog2e * (HALF ? __uint_as_float((uint32_t)(127 - 8 + e) << 23) : 1.0f);
-    }
-    if (lane == 0) {
-      int x0 = 0, x1 = 0;
-      if (on) row_range(a, s.pos + i, s.kv, x0, x1);
-      row_lo[r] = x0;
-      row_hi[r] = x1;
     }
   }
   __syncthreads();
@@ -353,38 +452,32 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
     all_lo = row_lo[rt * 8 + rv - 1];
     all_hi = row_hi[rt * 8];
   }
-  const uint2 *qw = qs + (size_t)rt * NP * S::KSTEPS * 32 + lane;
 
   float o[HD / 16][4];
 #pragma unroll
   for (int i = 0; i < HD / 16; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
 
-  bool bad = false;   // a wait gave up: go on without waiting (the call is reported as not complete)
-  auto wait = [&](uint64_t *bar, uint32_t parity) {
-    if (!bad && !mbar_wait(bar, parity)) bad = true;
-  };
   // This warp is done with unit u; the first warp of the group asks for the unit that takes its place.
   auto release = [&](int u) {
     __syncwarp();
     if (RT > 1) {
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&empty[u % D])) : "memory");
-      if (rt == 0 && (u + D) >> 1 < mine) wait(&empty[u % D], (uint32_t)((u / D) & 1));
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&empty[(ubase + u) % D])) : "memory");
+      if (rt == 0 && (u + D) >> 1 < mine) wait(&empty[(ubase + u) % D], (uint32_t)(((ubase + u) / D) & 1));
       __syncwarp();
     }
     if (rt == 0) request(u + D);
   };
-  auto lds16 = [](const uint8_t *at) { return *reinterpret_cast<const uint4 *>(at); };
 
 #pragma unroll 1
   for (int n = 0; n < mine; n++) {
-    const int uk = 2 * n, uv = 2 * n + 1;
+    const int uk = 2 * n, uv = 2 * n + 1, sk = (ubase + uk) % D, sv = (ubase + uv) % D;
     const int pos0 = (tile0 + tg + TG * n) * 16;
-    wait(&full[uk % D], (uint32_t)((uk / D) & 1));
-    const bool on = has[uk % D];
-    float sa[4] = {0, 0, 0, 0}, sb[4] = {0, 0, 0, 0};
+    wait(&full[sk], (uint32_t)(((ubase + uk) / D) & 1));
+    const bool on = has[sk];
+    float sc[4][4] = {};
     float ks0 = 1.0f, ks1 = 1.0f, w0 = 1.0f, w1 = 1.0f;
-    const uint8_t *unit = ring + (uk % D) * S::UNIT;
+    const uint8_t *unit = ring + sk * S::UNIT;
     if (on) {
       const uint8_t *kp = unit + g * S::ROW + c * 16;
       if (HALF) {
@@ -414,18 +507,17 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
 #pragma unroll
           for (int k = 0; k < NP; k++) {
             const uint2 bq = qw[(k * S::KSTEPS + m * ST + j) * 32];
-            if (j & 1)
-              mma16816<HALF>(sb, a0, a1, a2, a3, bq.x, bq.y);
-            else
-              mma16816<HALF>(sa, a0, a1, a2, a3, bq.x, bq.y);
+            mma16816<HALF>(sc[(m * ST + j) & 3], a0, a1, a2, a3, bq.x, bq.y);
           }
         }
       }
     }
     release(uk);
-    // ---- softmax of the tile: sa[0], sa[1] are position g of rows 2c, 2c + 1; sa[2], sa[3] g + 8.
-    float s0 = (sa[0] + sb[0]) * (ks0 * qf0), s1 = (sa[1] + sb[1]) * (ks0 * qf1);
-    float s2 = (sa[2] + sb[2]) * (ks1 * qf0), s3 = (sa[3] + sb[3]) * (ks1 * qf1);
+    // ---- softmax of the tile: sums 0, 1 are position g of rows 2c, 2c + 1; 2, 3 position g + 8.
+    float sa[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) sa[i] = (sc[0][i] + sc[1][i]) + (sc[2][i] + sc[3][i]);
+    float s0 = sa[0] * (ks0 * qf0), s1 = sa[1] * (ks0 * qf1), s2 = sa[2] * (ks1 * qf0), s3 = sa[3] * (ks1 * qf1);
     bool see0 = on, see1 = on, see2 = on, see3 = on;
     const bool whole = on && pos0 >= all_lo && pos0 + 16 <= all_hi;
     uint32_t dead = 0;   // positions that no row of the warp sees
@@ -485,9 +577,9 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
         pw[1][k] = transpose8x8(y[k]);
       }
     }
-    wait(&full[uv % D], (uint32_t)((uv / D) & 1));
+    wait(&full[sv], (uint32_t)(((ubase + uv) / D) & 1));
     if (on) {
-      const uint8_t *vp = ring + (uv % D) * S::UNIT + 2 * c * S::ROW + g * (S::NARROW ? 8 : 16);
+      const uint8_t *vp = ring + sv * S::UNIT + 2 * c * S::ROW + g * (S::NARROW ? 8 : 16);
       uint32_t odd = 0;   // bf16 pages: this lane met a value that is not finite at its i-th position
       constexpr int MM = S::NARROW ? 1 : S::ROW / 128;
 #pragma unroll
@@ -572,7 +664,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
   if (bad) {
     paged_raise(a.err, G4_PAGED_TIMEOUT);
     // What was asked for has landed, or a second limit has passed, before the ring is given up.
-    for (int u = 2 * mine > D ? 2 * mine - D : 0; u < 2 * mine; u++) mbar_wait(&full[u % D], (uint32_t)((u / D) & 1));
+    for (int u = 2 * mine > D ? 2 * mine - D : 0; u < 2 * mine; u++) mbar_wait(&full[(ubase + u) % D], (uint32_t)(((ubase + u) / D) & 1));
   }
 
   // ---- join the token groups through shared memory (over Q), then write out or leave a partial.
@@ -601,11 +693,11 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
     sm[ROWS * HD + ROWS + rt * 8 + 2 * c + 1] = l1;
   }
   __syncthreads();
-  __shared__ float fsh[(kJoin + 1) * ROWS];
-  __shared__ bool is_last;
   const float bits = HALF ? kWeightBits : 0.0f;
-  const long long slot0 = (((long long)b * p.kv_heads + kvh) * a.row_groups + rg) * a.splits;
-  float *mine_part = ns > 1 ? a.part + (slot0 + split) * PART : nullptr;
+  // Partial slots: 2 i for a part that block i begins inside of, 2 i + 1 for one it begins and leaves.
+  const int c_first = (int)(item_at / share), c_last = (int)((item_at + tiles - 1) / share), me = blockIdx.x;
+  auto slot_of = [&](int i) { return i == c_first ? 2 * i + 1 : 2 * i; };
+  float *mine_part = complete ? nullptr : a.part + (long long)slot_of(me) * PART;
   {
     // The same join as between blocks, its partials in shared memory.
     const float *sp = reinterpret_cast<const float *>(dsm);
@@ -656,37 +748,50 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
       }
     }
   }
-  if (ns == 1) return;
-
-  // ---- the last of each group of kJoin splits joins it; the last group joins the groups.
-  const int groups = (ns + kJoin - 1) / kJoin, grp = split / kJoin;
-  const int in_group = min(kJoin, ns - grp * kJoin);
-  const int max_groups = (a.splits + kJoin - 1) / kJoin;
-  uint32_t *cnt = a.count + (slot0 / a.splits) * (max_groups + 1);
-  __threadfence();
-  __syncthreads();
-  if (t == 0) {
-    is_last = atomicAdd(cnt + 1 + grp, 1u) == (unsigned)in_group - 1;
-    if (is_last) cnt[1 + grp] = 0;
+  if (!complete) {
+    // ---- the last of each kJoin neighbours joins them; the last of those the whole.
+    const int parts = c_last - c_first + 1, groups = (parts + kJoin - 1) / kJoin, grp = (me - c_first) / kJoin;
+    const int g0 = c_first + grp * kJoin, in_group = min(kJoin, parts - grp * kJoin);
+    uint32_t *group_count = a.count + 2 * slot_of(g0), *all_count = a.count + 2 * slot_of(c_first) + 1;
+    __threadfence();
+    __syncthreads();
+    if (t == 0) {
+      const bool last = atomicAdd(group_count, 1u) == (unsigned)in_group - 1;
+      if (last) *group_count = 0;
+      sum_sh[1] = last;
+    }
+    __syncthreads();
+    if (sum_sh[1]) {
+      __threadfence();
+      // Slots of a group's members are 2 PART apart from the second on; the first one's place differs.
+      float *base = a.part + (long long)slot_of(g0) * PART;
+      join_partials<HD>(a, base, in_group > 1 ? a.part + (long long)slot_of(g0 + 1) * PART : nullptr, 2ll * PART, in_group, ROWS,
+                        groups > 1 ? base : nullptr, s, kvh, row0, bits, fsh);
+      if (groups > 1) {
+        __threadfence();
+        __syncthreads();
+        if (t == 0) {
+          const bool last = atomicAdd(all_count, 1u) == (unsigned)groups - 1;
+          if (last) *all_count = 0;
+          sum_sh[2] = last;
+        }
+        __syncthreads();
+        if (sum_sh[2]) {
+          __threadfence();
+          join_partials<HD>(a, a.part + (long long)slot_of(c_first) * PART, a.part + (long long)slot_of(c_first + kJoin) * PART,
+                            2ll * kJoin * PART, groups, ROWS, nullptr, s, kvh, row0, bits, fsh);
+        }
+      }
+    }
   }
-  __syncthreads();
-  if (!is_last) return;
-  __threadfence();
-  float *base = a.part + (slot0 + (long long)grp * kJoin) * PART;
-  // A group's result replaces its first partial: each thread reads an element of all before it
-  // writes it, and the rows' statistics go through fsh.
-  join_partials<HD>(a, base, PART, in_group, ROWS, groups > 1 ? base : nullptr, s, kvh, row0, bits, fsh);
-  if (groups == 1) return;
-  __threadfence();
-  __syncthreads();
-  if (t == 0) {
-    is_last = atomicAdd(cnt, 1u) == (unsigned)groups - 1;
-    if (is_last) cnt[0] = 0;
+  ubase += 2 * mine;
+  at += count;
+  if (at < end) {
+    // The next part's positions come over what this one's partials took up.
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
   }
-  __syncthreads();
-  if (!is_last) return;
-  __threadfence();
-  join_partials<HD>(a, a.part + slot0 * PART, (long long)kJoin * PART, groups, ROWS, nullptr, s, kvh, row0, bits, fsh);
+  }
 }
 
 // ------------------------------------------------------------------------------ launch
@@ -699,37 +804,19 @@ static int decode_rt(const PagedAttn &a) {
   return R <= 8 ? 1 : (R <= 16 ? 2 : 4);
 }
 
-// Fills in the split: enough blocks for two rounds of the SMs, no split below one tile a warp, at most
-// kJoin^2 of them.
+static_assert(4 * 148 * 4 <= kPagedCounters, "two counters a partial, two partials a block");
+
+// Tiles a warp group works on before a share is split further.
 static void plan_decode(PagedAttn &a) {
-  const int rt = decode_rt(a), rows = 8 * rt, tg = kDecWarps / rt;
+  const int rt = decode_rt(a), rows = 8 * rt;
   a.row_groups = (int)(((long long)a.max_q * a.group + rows - 1) / rows);
-  // Positions a row group can see: its queries' windows, from a tile boundary.
-  long long span = a.max_kv;
-  if (a.window > 0) {
-    const long long w = (long long)a.window + (rows + a.group - 1) / a.group + 16;
-    if (w < span) span = w;
-  }
-  const int tiles = (int)((span + 15) / 16) > 0 ? (int)((span + 15) / 16) : 1;
-  const long long base = (long long)a.batch * a.pool.kv_heads * a.row_groups;
-  const int occ = 2;
-  long long want = (2ll * 148 * occ + base - 1) / base;
-  const long long most = (tiles + tg - 1) / tg;
-  if (want > most) want = most;
-  if (want > kJoin * kJoin) want = kJoin * kJoin;
-  if (base * (want / kJoin + 2) > kPagedCounters) want = 1;
-  int per = (int)((tiles + want - 1) / want);
-  per = (per + tg - 1) / tg * tg;
-  a.split_tiles = per;
-  a.splits = (tiles + per - 1) / per;
+  a.split_tiles = 2 * kDecWarps / rt;
 }
 
 size_t paged_attention_partials(const PagedAttn &args) {
   PagedAttn a = args;
   if (a.max_q < 1 || a.batch < 1 || chunk_path(a)) return 0;
-  plan_decode(a);
-  if (a.splits == 1) return 0;
-  return (size_t)a.batch * a.pool.kv_heads * a.row_groups * a.splits * (8 * decode_rt(a)) * (a.pool.hd + 2) * sizeof(float);
+  return (size_t)2 * 148 * most_blocks(a.pool.hd) * (8 * decode_rt(a)) * (a.pool.hd + 2) * sizeof(float);
 }
 
 template <int FMT, int HD, int NP, int RT>
@@ -740,8 +827,12 @@ static cudaError_t launch_decode_rt(const PagedAttn &a, cudaStream_t st) {
   cudaError_t e = cudaSuccess;
   once([&] { e = cudaFuncSetAttribute(k_paged_decode<FMT, HD, NP, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); });
   if (e != cudaSuccess) return e;
-  const dim3 grid(a.row_groups * a.pool.kv_heads, a.splits, a.batch);
-  return launch_k(k_paged_decode<FMT, HD, NP, RT>, grid, dim3(kDecWarps * 32), SMEM, st, false, a);
+  // As many blocks as the SMs hold at once, or as there can be shares.
+  long long span = a.max_kv;
+  if (a.window > 0) span = std::min<long long>(span, (long long)a.window + (8 * RT + a.group - 1) / a.group + 16);
+  const long long most = (long long)a.batch * a.pool.kv_heads * a.row_groups * std::max<long long>(1, (span + 15) / 16);
+  const long long blocks = std::min<long long>((most + a.split_tiles - 1) / a.split_tiles, 148 * S::OCC);
+  return launch_k(k_paged_decode<FMT, HD, NP, RT>, dim3((unsigned)blocks), dim3(kDecWarps * 32), SMEM, st, false, a);
 }
 template <int FMT, int HD, int NP>
 static cudaError_t launch_decode_np(const PagedAttn &a, cudaStream_t st) {

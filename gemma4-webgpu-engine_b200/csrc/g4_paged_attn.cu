@@ -128,7 +128,10 @@ struct DecShape {
   static constexpr int UNIT = 16 * ROW + (HALF ? 128 : 0);   // K's (with both scales) or V's 16 positions
   static constexpr int Q_BYTES = RT * NP * KSTEPS * 32 * 8;
   // Blocks on an SM: as many as the registers allow (O takes HD / 4 of them) with three units a ring.
-  static constexpr int ring_depth(int occ) { return ((occ == 1 ? 220 : 216 / occ) * 1024 - 1024 * 4 - Q_BYTES) / (TG * UNIT); }
+  // (228 KB of shared memory an SM, 1 KB a block the system's; the arrays besides Q and ring.)
+  static constexpr int ring_depth(int occ) {
+    return ((occ == 1 ? 227 : 228 / occ - 1) * 1024 - 1536 - (kJoin + 1) * 8 * RT * 4 - Q_BYTES) / (TG * UNIT);
+  }
   static constexpr int MOST = most_blocks(HD);
   static constexpr int OCC = ring_depth(MOST) >= 3 ? MOST : (ring_depth(2) >= 3 ? 2 : 1);
   static constexpr int DD = ring_depth(OCC), D = DD > 8 ? 8 : DD;
@@ -274,7 +277,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
   if (before <= at && at < before + mine_sum) {
     long long x = before;
     int b = t * per;
-    for (;; b++) {
+    for (; per > 1; b++) {
       const long long n = seq_tiles(b, false);
       if (at < x + n) break;
       x += n;
@@ -332,14 +335,20 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
   // ---- this group's tiles: tile0 + tg + TG n; its first warp asks for them.
   const int mine = tile1 - tile0 - tg > 0 ? (tile1 - tile0 - tg + TG - 1) / TG : 0;
   const int32_t *table = a.table + (long long)b * a.table_stride;
-  // Lane i of the first warp holds the page of the i-th of 32 tiles from pages_at on (-1: none).
-  int pages = -1, pages_at = 0;
+  // Lane i of the first warp holds where the rows of the i-th of 32 tiles from pages_at on lie in the
+  // pool (-1: no such page), so that asking for one is a shuffle and the copies.
+  long long rows = -1;
+  int pages_at = 0;
   auto fetch_pages = [&](int n) {
     const int k = n + lane;
-    pages = k < mine ? table[(tile0 + tg + TG * k) / per_page] : -1;
-    if (k < mine && (pages < 0 || pages >= p.n_pages)) {
-      paged_raise(a.err, G4_PAGED_BAD_PAGE);
-      pages = -1;
+    rows = -1;
+    if (k < mine) {
+      const int tile = tile0 + tg + TG * k, of = tile / per_page;
+      const int page = table[of];
+      if (page < 0 || page >= p.n_pages)
+        paged_raise(a.err, G4_PAGED_BAD_PAGE);
+      else
+        rows = ((long long)page * p.kv_heads + kvh) * p.page_size + (tile - of * per_page) * 16;
     }
     pages_at = n;
   };
@@ -370,29 +379,30 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
   load_q(warp, qv[0]);
   load_q(warp + kDecWarps, qv[1]);
 
-  // Unit u of the group (K of tile u / 2, or V), by its whole first warp.
-  auto request = [&](int u) {
-    const int n = u >> 1, sl = (ubase + u) % D;
+  // Unit u of the group (K of tile u / 2, or V) into slot sl, by its whole first warp.
+  auto request = [&](int u, int sl) {
+    const int n = u >> 1;
     if (n >= mine) return;
     if (n - pages_at >= 32) fetch_pages(n);
-    const int page = __shfl_sync(0xffffffffu, pages, n - pages_at);
+    const long long row = __shfl_sync(0xffffffffu, rows, n - pages_at);
     if (lane != 0) return;
-    has[sl] = page >= 0;
-    if (page < 0) {
+    has[sl] = row >= 0;
+    if (row < 0) {
       asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&full[sl])) : "memory");
       return;
     }
-    const long long row = ((long long)page * p.kv_heads + kvh) * p.page_size + ((tile0 + tg + TG * n) % per_page) * 16;
     uint8_t *to = ring + sl * S::UNIT;
-    mbar_expect_tx(&full[sl], 16 * S::ROW + (HALF && !(u & 1) ? 128 : 0));
-    bulk_g2s(to, (u & 1 ? p.v : p.k) + row * S::ROW, 16 * S::ROW, &full[sl]);
-    if (HALF && !(u & 1)) {
+    const bool is_v = u & 1;
+    mbar_expect_tx(&full[sl], 16 * S::ROW + (HALF && !is_v ? 128 : 0));
+    bulk_g2s(to, (is_v ? p.v : p.k) + row * S::ROW, 16 * S::ROW, &full[sl]);
+    if (HALF && !is_v) {
       bulk_g2s(to + 16 * S::ROW, p.ks + row, 64, &full[sl]);
       bulk_g2s(to + 16 * S::ROW + 64, p.vs + row, 64, &full[sl]);
     }
   };
+  const int sl0 = ubase % D;   // the first unit's slot
   if (rt == 0)
-    for (int u = 0; u < D; u++) request(u);
+    for (int u = 0; u < D; u++) request(u, sl0 + u < D ? sl0 + u : sl0 + u - D);
 
   // Q into fragment order: for K step k of row tile r lane (g, c) holds four consecutive dimensions of
   // row g. 8-bit pages: f16 parts, scaled by a power of two that takes the row's greatest to 2^8 .. 2^9.
@@ -458,26 +468,34 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
   for (int i = 0; i < HD / 16; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
 
-  // This warp is done with unit u; the first warp of the group asks for the unit that takes its place.
-  auto release = [&](int u) {
+  // This warp is done with unit u in slot sl; the first warp of the group asks for the unit that takes its
+  // place.
+  auto release = [&](int u, int sl, uint32_t round) {
     __syncwarp();
     if (RT > 1) {
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&empty[(ubase + u) % D])) : "memory");
-      if (rt == 0 && (u + D) >> 1 < mine) wait(&empty[(ubase + u) % D], (uint32_t)(((ubase + u) / D) & 1));
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&empty[sl])) : "memory");
+      if (rt == 0 && (u + D) >> 1 < mine) wait(&empty[sl], round);
       __syncwarp();
     }
-    if (rt == 0) request(u + D);
+    if (rt == 0) request(u + D, sl);
+  };
+  int sl = sl0;                                       // the ring's slot at hand and its round
+  uint32_t round = (uint32_t)(ubase / D) & 1;
+  auto advance = [&] {
+    if (++sl == D) {
+      sl = 0;
+      round ^= 1;
+    }
   };
 
 #pragma unroll 1
   for (int n = 0; n < mine; n++) {
-    const int uk = 2 * n, uv = 2 * n + 1, sk = (ubase + uk) % D, sv = (ubase + uv) % D;
     const int pos0 = (tile0 + tg + TG * n) * 16;
-    wait(&full[sk], (uint32_t)(((ubase + uk) / D) & 1));
-    const bool on = has[sk];
+    wait(&full[sl], round);
+    const bool on = has[sl];
     float sc[4][4] = {};
     float ks0 = 1.0f, ks1 = 1.0f, w0 = 1.0f, w1 = 1.0f;
-    const uint8_t *unit = ring + sk * S::UNIT;
+    const uint8_t *unit = ring + sl * S::UNIT;
     if (on) {
       const uint8_t *kp = unit + g * S::ROW + c * 16;
       if (HALF) {
@@ -512,7 +530,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
         }
       }
     }
-    release(uk);
+    release(2 * n, sl, round);
+    advance();
     // ---- softmax of the tile: sums 0, 1 are position g of rows 2c, 2c + 1; 2, 3 position g + 8.
     float sa[4];
 #pragma unroll
@@ -577,9 +596,9 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
         pw[1][k] = transpose8x8(y[k]);
       }
     }
-    wait(&full[sv], (uint32_t)(((ubase + uv) / D) & 1));
+    wait(&full[sl], round);
     if (on) {
-      const uint8_t *vp = ring + sv * S::UNIT + 2 * c * S::ROW + g * (S::NARROW ? 8 : 16);
+      const uint8_t *vp = ring + sl * S::UNIT + 2 * c * S::ROW + g * (S::NARROW ? 8 : 16);
       uint32_t odd = 0;   // bf16 pages: this lane met a value that is not finite at its i-th position
       constexpr int MM = S::NARROW ? 1 : S::ROW / 128;
 #pragma unroll
@@ -659,7 +678,8 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
         if ((b0 && see1) || (b1 && see3)) l1 = nan;
       }
     }
-    release(uv);
+    release(2 * n + 1, sl, round);
+    advance();
   }
   if (bad) {
     paged_raise(a.err, G4_PAGED_TIMEOUT);

@@ -11,6 +11,8 @@
 #include <cuda_runtime.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "g4_device.cuh"
 #include "g4_kernels.cuh"
 #include "g4_paged.cuh"
@@ -18,6 +20,13 @@
 namespace g4 {
 
 constexpr int kDraftThreads = 256;
+constexpr float kLog2e = 1.44269504088896341f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 struct Race {
   float key;
@@ -151,21 +160,23 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_scan(const DraftArgs a,
   const float *noise = a.gumbel + (long long)b * a.ld_gumbel;
   RowSum sum{-INFINITY, 0.0f};
   Race best{-INFINITY, 0x7fffffff};
-  const int c1 = min(a.vocab, (split + 1) * a.chunk);
-  constexpr int U = 16 / VEC;   // loads in flight of each kind
-  for (int i0 = split * a.chunk + t * VEC; i0 < c1; i0 += kDraftThreads * VEC * U) {
+  const int c0 = split * a.chunk, c1 = min(a.vocab, c0 + a.chunk);
+  constexpr int U = 16 / VEC, STEP = kDraftThreads * VEC;   // loads in flight of each kind
+  // One pass of 16 tokens a thread. FULL: all of them are there and none is left out.
+  auto pass = [&](auto full_, auto race_, auto noisy_, int i0) {
+    constexpr bool FULL = decltype(full_)::value, RACE = decltype(race_)::value, NOISY = decltype(noisy_)::value;
     float x[U][VEC], g[U][VEC];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int i = i0 + u * kDraftThreads * VEC;
-      if (i + VEC <= c1) {
+      const int i = i0 + u * STEP;
+      if (FULL || i + VEC <= c1) {
         load_vec<T, VEC>(src + i, x[u]);
-        if (noisy) load_vec<float, VEC>(noise + i, g[u]);
+        if (NOISY) load_vec<float, VEC>(noise + i, g[u]);
       } else {
 #pragma unroll
         for (int e = 0; e < VEC; e++) {
           x[u][e] = i + e < c1 ? logit_at<T>(a, row, i + e) : -INFINITY;
-          g[u][e] = noisy && i + e < c1 ? noise[i + e] : 0.0f;
+          g[u][e] = NOISY && i + e < c1 ? noise[i + e] : 0.0f;
         }
       }
     }
@@ -177,21 +188,36 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_scan(const DraftArgs a,
         x[u][e] = __fmul_rn(x[u][e], inv);
         top = fmaxf(top, x[u][e]);
       }
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float s = sum.s * __expf(sum.m - ref);
+    const float ref = top == -INFINITY ? 0.0f : top, low = -ref * kLog2e;
+    float s0 = sum.s * ex2(fmaf(sum.m, kLog2e, low)), s1 = 0.0f;
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
       for (int e = 0; e < VEC; e++) {
-        s += __expf(x[u][e] - ref);
-        if (race) {
-          const int i = i0 + u * kDraftThreads * VEC + e;
-          const float key = noisy ? __fadd_rn(x[u][e], g[u][e]) : x[u][e];
-          if (key > best.key && i != left_out) best = {key, i};
+        ((u * VEC + e) & 1 ? s1 : s0) += ex2(fmaf(x[u][e], kLog2e, low));
+        if (RACE) {
+          const int i = i0 + u * STEP + e;
+          const float key = NOISY ? __fadd_rn(x[u][e], g[u][e]) : x[u][e];
+          if (key > best.key && (FULL || i != left_out)) best = {key, i};
         }
       }
-    sum = {top, s};
-  }
+    sum = {top, s0 + s1};
+  };
+  auto passes = [&](auto race_, auto noisy_) {
+    for (int b0 = c0; b0 < c1; b0 += STEP * U) {
+      const int i0 = b0 + t * VEC;
+      if (b0 + STEP * U <= c1 && (left_out < b0 || left_out >= b0 + STEP * U))
+        pass(std::true_type{}, race_, noisy_, i0);
+      else
+        pass(std::false_type{}, race_, noisy_, i0);
+    }
+  };
+  if (noisy)
+    passes(std::true_type{}, std::true_type{});
+  else if (race)
+    passes(std::true_type{}, std::false_type{});
+  else
+    passes(std::false_type{}, std::false_type{});
   DraftPart v = block_join({sum.m, sum.s, best.key, best.idx}, sh);
   DraftPart *parts = a.part + ((long long)b * width + j) * a.splits;
   if (t == 0) {

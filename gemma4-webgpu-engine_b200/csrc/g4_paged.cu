@@ -8,6 +8,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <type_traits>
 
 #include "g4_device.cuh"
 #include "g4_kernels.cuh"
@@ -116,74 +117,83 @@ __device__ __forceinline__ void decode8(uint2 c, float s, float (&x)[8]) {
   }
 }
 
+constexpr int kRowItems = 2;   // (token, head) pairs a thread has in flight
+
 template <typename T, int FMT, int HD>
 __global__ void __launch_bounds__(256)
     k_page_store(const Pool p, const T *__restrict__ k, const T *__restrict__ v, long long k_stride,
                  long long v_stride, int tokens, const int32_t *__restrict__ slots) {
   constexpr int LR = HD / 8 < 32 ? HD / 8 : 32;   // lanes per row
   constexpr int CH = HD / 8 / LR;                 // chunks of eight per lane
-  const long long item = ((long long)blockIdx.x * 256 + threadIdx.x) / LR;
+  constexpr int IPB = 256 / LR;                   // items a block takes side by side
   const int l = threadIdx.x % LR;
   const long long items = (long long)tokens * p.kv_heads;
-  const bool live = item < items;
-  const int tok = live ? (int)(item / p.kv_heads) : 0, head = live ? (int)(item % p.kv_heads) : 0;
-  int slot = live ? slots[tok] : -1;
-  if (slot >= p.n_pages * p.page_size) {
-    if (l == 0) paged_raise(&g4_paged_error, G4_PAGED_BAD_PAGE);
-    slot = -1;
-  }
-  const bool on = slot >= 0;
-  Eight<T> in[2][CH];
-  if (on) {
+  Eight<T> in[kRowItems][2][CH];
+  int slot[kRowItems], head[kRowItems];
+#pragma unroll
+  for (int n = 0; n < kRowItems; n++) {
+    const long long item = ((long long)blockIdx.x * kRowItems + n) * IPB + threadIdx.x / LR;
+    const bool live = item < items;
+    const int tok = live ? (int)(item / p.kv_heads) : 0;
+    head[n] = live ? (int)(item - (long long)tok * p.kv_heads) : 0;
+    slot[n] = live ? slots[tok] : -1;
+    // (The rows are there whatever the slot: their loads do not wait for it.)
 #pragma unroll
     for (int c = 0; c < CH; c++) {
-      in[0][c].load(k + tok * k_stride + head * HD + (c * LR + l) * 8);
-      in[1][c].load(v + tok * v_stride + head * HD + (c * LR + l) * 8);
+      in[n][0][c].load(k + tok * k_stride + head[n] * HD + (c * LR + l) * 8);
+      in[n][1][c].load(v + tok * v_stride + head[n] * HD + (c * LR + l) * 8);
     }
   }
-  const int page = on ? slot / p.page_size : 0, off = on ? slot - page * p.page_size : 0;
-  const long long row = ((long long)page * p.kv_heads + head) * p.page_size + off;
 #pragma unroll
-  for (int w = 0; w < 2; w++) {
-    uint8_t *const base = w ? p.v : p.k;
-    if (FMT == G4_PAGE_BF16) {
+  for (int n = 0; n < kRowItems; n++) {
+    if (slot[n] >= p.n_pages * p.page_size) {
+      if (l == 0) paged_raise(&g4_paged_error, G4_PAGED_BAD_PAGE);
+      slot[n] = -1;
+    }
+    const bool on = slot[n] >= 0;
+    const int page = on ? slot[n] / p.page_size : 0, off = on ? slot[n] - page * p.page_size : 0;
+    const long long row = ((long long)page * p.kv_heads + head[n]) * p.page_size + off;
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+      uint8_t *const base = w ? p.v : p.k;
+      if (FMT == G4_PAGE_BF16) {
+        if (on) {
+#pragma unroll
+          for (int c = 0; c < CH; c++) {
+            float x[8];
+            in[n][w][c].get(x);
+            Eight<__nv_bfloat16>::put(reinterpret_cast<__nv_bfloat16 *>(base) + row * HD + (c * LR + l) * 8, x);
+          }
+        }
+        continue;
+      }
+      // The greatest magnitude over the row; x - x is 0 unless x is an infinity or a NaN.
+      float top = 0.0f;
+      bool bad = false;
+#pragma unroll
+      for (int c = 0; c < CH; c++) {
+        float x[8];
+        in[n][w][c].get(x);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          top = fmaxf(top, fabsf(x[i]));
+          bad |= !(__fsub_rn(x[i], x[i]) == 0.0f);
+        }
+      }
+      if (bad) top = __int_as_float(0x7f800000);
+#pragma unroll
+      for (int m = 1; m < LR; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+      float s = __fdiv_rn(top, FMT == G4_PAGE_INT8 ? 127.0f : 448.0f);
+      if (s == __int_as_float(0x7f800000)) s = __int_as_float(0x7fffffff);
       if (on) {
 #pragma unroll
         for (int c = 0; c < CH; c++) {
           float x[8];
-          in[w][c].get(x);
-          Eight<__nv_bfloat16>::put(reinterpret_cast<__nv_bfloat16 *>(base) + row * HD + (c * LR + l) * 8, x);
+          in[n][w][c].get(x);
+          *reinterpret_cast<uint2 *>(base + row * HD + (c * LR + l) * 8) = encode8<FMT>(x, s);
         }
+        if (l == 0) (w ? p.vs : p.ks)[row] = s;
       }
-      continue;
-    }
-    // The greatest magnitude over the row; x - x is 0 unless x is an infinity or a NaN.
-    float top = 0.0f;
-    bool bad = false;
-#pragma unroll
-    for (int c = 0; c < CH; c++) {
-      float x[8];
-      in[w][c].get(x);
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        if (!on) x[i] = 0.0f;
-        top = fmaxf(top, fabsf(x[i]));
-        bad |= !(__fsub_rn(x[i], x[i]) == 0.0f);
-      }
-    }
-    if (bad) top = __int_as_float(0x7f800000);
-#pragma unroll
-    for (int m = 1; m < LR; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-    float s = __fdiv_rn(top, FMT == G4_PAGE_INT8 ? 127.0f : 448.0f);
-    if (s == __int_as_float(0x7f800000)) s = __int_as_float(0x7fffffff);
-    if (on) {
-#pragma unroll
-      for (int c = 0; c < CH; c++) {
-        float x[8];
-        in[w][c].get(x);
-        *reinterpret_cast<uint2 *>(base + row * HD + (c * LR + l) * 8) = encode8<FMT>(x, s);
-      }
-      if (l == 0) (w ? p.vs : p.ks)[row] = s;
     }
   }
 }
@@ -194,53 +204,55 @@ __global__ void __launch_bounds__(256)
                 int tokens, const int32_t *__restrict__ slots) {
   constexpr int LR = HD / 8 < 32 ? HD / 8 : 32;
   constexpr int CH = HD / 8 / LR;
-  const long long item = ((long long)blockIdx.x * 256 + threadIdx.x) / LR;
+  constexpr int IPB = 256 / LR;
   const int l = threadIdx.x % LR;
-  if (item >= (long long)tokens * p.kv_heads) return;
-  const int tok = (int)(item / p.kv_heads), head = (int)(item % p.kv_heads);
-  int slot = slots[tok];
-  if (slot >= p.n_pages * p.page_size) {
-    if (l == 0) paged_raise(&g4_paged_error, G4_PAGED_BAD_PAGE);
-    slot = -1;
-  }
-  const bool on = slot >= 0;
-  const int page = on ? slot / p.page_size : 0, off = on ? slot - page * p.page_size : 0;
-  const long long row = ((long long)page * p.kv_heads + head) * p.page_size + off;
-  float x[2][CH][8];
-  if (FMT == G4_PAGE_BF16) {
-    Eight<__nv_bfloat16> in[2][CH];
+  const long long items = (long long)tokens * p.kv_heads;
+  using Code = typename std::conditional<FMT == G4_PAGE_BF16, uint4, uint2>::type;   // eight of them
+  constexpr int ES = FMT == G4_PAGE_BF16 ? 2 : 1;
+  Code in[kRowItems][2][CH];
+  float s[kRowItems][2];
+  int tok[kRowItems], head[kRowItems];
 #pragma unroll
-    for (int w = 0; w < 2; w++)
-#pragma unroll
-      for (int c = 0; c < CH; c++) {
-        in[w][c].a = make_uint4(0, 0, 0, 0);
-        if (on) in[w][c].load(reinterpret_cast<const __nv_bfloat16 *>(w ? p.v : p.k) + row * HD + (c * LR + l) * 8);
-      }
-#pragma unroll
-    for (int w = 0; w < 2; w++)
-#pragma unroll
-      for (int c = 0; c < CH; c++) in[w][c].get(x[w][c]);
-  } else {
-    uint2 in[2][CH];
-    float s[2] = {0.0f, 0.0f};
+  for (int n = 0; n < kRowItems; n++) {
+    const long long item = ((long long)blockIdx.x * kRowItems + n) * IPB + threadIdx.x / LR;
+    tok[n] = item < items ? (int)(item / p.kv_heads) : -1;
+    head[n] = item < items ? (int)(item - (long long)tok[n] * p.kv_heads) : 0;
+    int slot = tok[n] >= 0 ? slots[tok[n]] : -1;
+    if (slot >= p.n_pages * p.page_size) {
+      if (l == 0) paged_raise(&g4_paged_error, G4_PAGED_BAD_PAGE);
+      slot = -1;
+    }
+    const bool on = slot >= 0;
+    const int page = on ? slot / p.page_size : 0, off = on ? slot - page * p.page_size : 0;
+    const long long row = ((long long)page * p.kv_heads + head[n]) * p.page_size + off;
 #pragma unroll
     for (int w = 0; w < 2; w++) {
 #pragma unroll
       for (int c = 0; c < CH; c++) {
-        in[w][c] = make_uint2(0, 0);
-        if (on) in[w][c] = *reinterpret_cast<const uint2 *>((w ? p.v : p.k) + row * HD + (c * LR + l) * 8);
+        in[n][w][c] = Code{};
+        if (on) in[n][w][c] = *reinterpret_cast<const Code *>((w ? p.v : p.k) + (row * HD + (c * LR + l) * 8) * ES);
       }
-      if (on) s[w] = (w ? p.vs : p.ks)[row];
+      s[n][w] = 0.0f;
+      if (on && FMT != G4_PAGE_BF16) s[n][w] = (w ? p.vs : p.ks)[row];
     }
+  }
+#pragma unroll
+  for (int n = 0; n < kRowItems; n++) {
+    if (tok[n] < 0) continue;
 #pragma unroll
     for (int w = 0; w < 2; w++)
 #pragma unroll
-      for (int c = 0; c < CH; c++) decode8<FMT>(in[w][c], s[w], x[w][c]);
-  }
-#pragma unroll
-  for (int c = 0; c < CH; c++) {
-    Eight<T>::put(k + tok * k_stride + head * HD + (c * LR + l) * 8, x[0][c]);
-    Eight<T>::put(v + tok * v_stride + head * HD + (c * LR + l) * 8, x[1][c]);
+      for (int c = 0; c < CH; c++) {
+        float x[8];
+        if constexpr (FMT == G4_PAGE_BF16) {
+          Eight<__nv_bfloat16> e;
+          e.a = in[n][w][c];
+          e.get(x);
+        } else {
+          decode8<FMT>(in[n][w][c], s[n][w], x);
+        }
+        Eight<T>::put((w ? v + tok[n] * v_stride : k + tok[n] * k_stride) + head[n] * HD + (c * LR + l) * 8, x);
+      }
   }
 }
 
@@ -248,8 +260,8 @@ template <typename T, int FMT>
 cudaError_t launch_rows(const Pool &p, bool store, void *k, void *v, long long ks, long long vs, int tokens,
                         const int32_t *slots, cudaStream_t st) {
   const int lanes = p.hd / 8 < 32 ? p.hd / 8 : 32;
-  const long long threads = (long long)tokens * p.kv_heads * lanes;
-  const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
+  const long long per_block = 256 / lanes * kRowItems;
+  const dim3 grid((unsigned)(((long long)tokens * p.kv_heads + per_block - 1) / per_block)), block(256);
   T *tk = (T *)k, *tv = (T *)v;
   auto go = [&](auto hd) {
     constexpr int HD = decltype(hd)::value;

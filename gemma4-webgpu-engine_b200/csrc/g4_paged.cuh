@@ -28,9 +28,10 @@ struct PagedAttn {
   const int32_t *q_begin, *q_pos, *kv_len, *table;
   int table_stride, max_q, max_kv, window;
   float scale;
-  // Set by the launcher: the least tiles of 16 positions a block takes, the row groups per (sequence,
-  // KV head); the blocks' partials and the counts of finished ones.
-  int split_tiles, row_groups;
+  // Set by the launcher: the least tiles of 16 positions a block takes, the tiles that beginning a list
+  // item counts for, the row groups per (sequence, KV head); the blocks' partials and the counts of
+  // finished ones.
+  int split_tiles, begin_tiles, row_groups;
   float *part;
   uint32_t *count;
   int *err;

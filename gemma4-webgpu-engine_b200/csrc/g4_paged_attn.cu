@@ -38,6 +38,11 @@
 namespace g4 {
 
 constexpr int kDecWarps = 4;
+#ifndef SPLIT_T
+#define SPLIT_T 3
+#define BEGIN_T 16
+#endif
+constexpr int kRingKb = 96;          // of an SM's shared memory in rings
 constexpr int kJoin = 16;            // partials one block joins
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 constexpr float kWeightBits = 14.0f; // 8-bit codes: weights are scaled by 2^14, clear of f16's subnormals
@@ -133,8 +138,11 @@ struct DecShape {
     return ((occ == 1 ? 227 : 228 / occ - 1) * 1024 - 1536 - (kJoin + 1) * 8 * RT * 4 - Q_BYTES) / (TG * UNIT);
   }
   static constexpr int MOST = most_blocks(HD);
-  static constexpr int OCC = ring_depth(MOST) >= 3 ? MOST : (ring_depth(2) >= 3 ? 2 : 1);
-  static constexpr int DD = ring_depth(OCC), D = DD > 8 ? 8 : DD;
+  static constexpr int OCC = ring_depth(MOST) >= 2 ? MOST : (ring_depth(2) >= 2 ? 2 : 1);
+  // Deep enough for the bytes that HBM needs in flight and no deeper: the queue before the memory is
+  // what every other load of the block waits in.
+  static constexpr int WANT = kRingKb * 1024 / (OCC * TG * UNIT), CAP = ring_depth(OCC) > 8 ? 8 : ring_depth(OCC);
+  static constexpr int D = WANT < 2 ? 2 : (WANT > CAP ? CAP : WANT);
   static_assert(D >= 2, "a ring holds K and V of a tile");
   static constexpr int RING = TG * D * UNIT, JOIN = TG * 8 * RT * (HD + 2) * 4;
   static constexpr int SMEM = Q_BYTES + RING > JOIN ? Q_BYTES + RING : JOIN;
@@ -147,25 +155,32 @@ struct DecShape {
 template <int HD>
 __device__ __forceinline__ void join_partials(const PagedAttn &a, const float *first, const float *rest, long long stride, int np, int rows,
                                               float *to, const SeqSpan &s, int kvh, int row0, float bits, float *fsh) {
-  // fsh: [np][rows] factors, then [rows] 1 / l.
+  // fsh: [np][rows] factors, then [rows] l. Sixteen lanes a row, a partial each.
   const int t = threadIdx.x, nt = blockDim.x;
   auto part = [&](int i) { return i == 0 ? first : rest + (i - 1) * stride; };
-  for (int r = t; r < rows; r += nt) {
-    float M = -INFINITY;
-    for (int i = 0; i < np; i++) M = fmaxf(M, __ldcg(part(i) + rows * HD + r));
-    float l = 0.0f;
-    for (int i = 0; i < np; i++) {
-      const float m = __ldcg(part(i) + rows * HD + r);
-      fsh[i * rows + r] = M == -INFINITY ? 0.0f : ex2(m - M);
-      l += rescale(__ldcg(part(i) + rows * HD + rows + r), M == -INFINITY ? 0.0f : m - M);
+  static_assert(kJoin == 16, "half a warp a row");
+  for (int x = t; x < rows * kJoin; x += nt) {
+    const int r = x / kJoin, i = x % kJoin;
+    float m = -INFINITY, l = 0.0f;
+    if (i < np) {
+      m = __ldcg(part(i) + rows * HD + r);
+      l = __ldcg(part(i) + rows * HD + rows + r);
     }
+    float M = m;
+#pragma unroll
+    for (int d = 1; d < kJoin; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+    if (i < np) fsh[i * rows + r] = M == -INFINITY ? 0.0f : ex2(m - M);
+    l = i < np ? rescale(l, M == -INFINITY ? 0.0f : m - M) : 0.0f;
+#pragma unroll
+    for (int d = 1; d < kJoin; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    if (i != 0) continue;
     fsh[np * rows + r] = l;
-    const int rr = row0 + r, i = rr / a.group;
+    const int rr = row0 + r, j = rr / a.group;
     if (to) {
       to[rows * HD + r] = M;
       to[rows * HD + rows + r] = l;
-    } else if (a.lse && i < s.n) {
-      a.lse[(long long)(s.row + i) * a.heads + kvh * a.group + rr % a.group] =
+    } else if (a.lse && j < s.n) {
+      a.lse[(long long)(s.row + j) * a.heads + kvh * a.group + rr % a.group] =
           M == -INFINITY ? -INFINITY : (M - bits + log2f(l)) * kLn2;
     }
   }
@@ -174,14 +189,21 @@ __device__ __forceinline__ void join_partials(const PagedAttn &a, const float *f
     const int r = e / (HD / 4), d = e % (HD / 4) * 4, rr = row0 + r, i = rr / a.group;
     if (!to && i >= s.n) continue;
     float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll 8
-    for (int k = 0; k < np; k++) {
-      const float f = fsh[k * rows + r];
-      const float4 v = __ldcg(reinterpret_cast<const float4 *>(part(k) + r * HD + d));
-      o.x = fmaf(f, v.x, o.x);
-      o.y = fmaf(f, v.y, o.y);
-      o.z = fmaf(f, v.z, o.z);
-      o.w = fmaf(f, v.w, o.w);
+#pragma unroll
+    for (int k0 = 0; k0 < kJoin; k0 += 8) {
+      if (k0 >= np) break;
+      float4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        v[k] = k0 + k < np ? __ldcg(reinterpret_cast<const float4 *>(part(k0 + k) + r * HD + d)) : make_float4(0, 0, 0, 0);
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const float f = k0 + k < np ? fsh[(k0 + k) * rows + r] : 0.0f;
+        o.x = fmaf(f, v[k].x, o.x);
+        o.y = fmaf(f, v[k].y, o.y);
+        o.z = fmaf(f, v[k].z, o.z);
+        o.w = fmaf(f, v[k].w, o.w);
+      }
     }
     if (to) {
       *reinterpret_cast<float4 *>(to + r * HD + d) = o;
@@ -228,8 +250,9 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
     mbar_fence_init();
   }
 
-  // ---- the list. Tiles of row group rg of sequence s (one even where nothing is seen: zeros are
-  // written there), from its first.
+  // ---- the list. Tiles of row group rg of sequence s from its first one, and before them a.begin_tiles
+  // that stand for what beginning it costs (a second part of a block's share costs as much as so many
+  // tiles; where nothing is seen they are all there is, and zeros are written).
   auto tiles_of = [&](const SeqSpan &s, int rg, int &first) {
     const int R = s.n * a.group, r0 = rg * ROWS;
     if (r0 >= R) return 0;
@@ -237,7 +260,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
     row_range(a, s.pos + r0 / a.group, s.kv, lo, tmp);
     row_range(a, s.pos + (min(r0 + ROWS, R) - 1) / a.group, s.kv, tmp, hi);
     first = lo >> 4;
-    return hi > lo ? ((hi + 15) >> 4) - first : 1;
+    return (hi > lo ? ((hi + 15) >> 4) - first : 0) + a.begin_tiles;
   };
   // All tiles of sequence b.
   auto seq_tiles = [&](int b, bool report) -> long long {
@@ -321,16 +344,15 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
     }
   }
   const int R = s.n * a.group, row0 = rg * ROWS;
-  const int tile0 = first + (int)(at - item_at);
-  const int count = (int)min((long long)tiles - (at - item_at), end - at);
-  const bool complete = count == tiles;
-  int lo, hi;
-  {
-    int tmp;
-    row_range(a, s.pos + row0 / a.group, s.kv, lo, tmp);
-    row_range(a, s.pos + (min(row0 + ROWS, R) - 1) / a.group, s.kv, tmp, hi);
+  const int from = (int)(at - item_at), count = (int)min((long long)tiles - from, end - at);
+  // The share may end among the tiles that stand for the beginning: then there is nothing to do here.
+  const int begin = a.begin_tiles, real = tiles - begin;
+  const int tile0 = first + max(from - begin, 0), tile1 = first + max(from + count - begin, 0);
+  if (real > 0 && tile1 == tile0) {
+    at += count;
+    continue;
   }
-  const int tile1 = hi > lo ? tile0 + count : tile0;   // (nothing seen: no tile to read)
+  const bool complete = tile1 - tile0 == real;
 
   // ---- this group's tiles: tile0 + tg + TG n; its first warp asks for them.
   const int mine = tile1 - tile0 - tg > 0 ? (tile1 - tile0 - tg + TG - 1) / TG : 0;
@@ -715,7 +737,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
   __syncthreads();
   const float bits = HALF ? kWeightBits : 0.0f;
   // Partial slots: 2 i for a part that block i begins inside of, 2 i + 1 for one it begins and leaves.
-  const int c_first = (int)(item_at / share), c_last = (int)((item_at + tiles - 1) / share), me = blockIdx.x;
+  const int c_first = (int)((item_at + begin) / share), c_last = (int)((item_at + tiles - 1) / share), me = blockIdx.x;
   auto slot_of = [&](int i) { return i == c_first ? 2 * i + 1 : 2 * i; };
   float *mine_part = complete ? nullptr : a.part + (long long)slot_of(me) * PART;
   {
@@ -773,31 +795,31 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
     const int parts = c_last - c_first + 1, groups = (parts + kJoin - 1) / kJoin, grp = (me - c_first) / kJoin;
     const int g0 = c_first + grp * kJoin, in_group = min(kJoin, parts - grp * kJoin);
     uint32_t *group_count = a.count + 2 * slot_of(g0), *all_count = a.count + 2 * slot_of(c_first) + 1;
-    __threadfence();
     __syncthreads();
     if (t == 0) {
+      __threadfence();   // (orders what the barrier has ordered before it)
       const bool last = atomicAdd(group_count, 1u) == (unsigned)in_group - 1;
+      __threadfence();
       if (last) *group_count = 0;
       sum_sh[1] = last;
     }
     __syncthreads();
     if (sum_sh[1]) {
-      __threadfence();
       // Slots of a group's members are 2 PART apart from the second on; the first one's place differs.
       float *base = a.part + (long long)slot_of(g0) * PART;
       join_partials<HD>(a, base, in_group > 1 ? a.part + (long long)slot_of(g0 + 1) * PART : nullptr, 2ll * PART, in_group, ROWS,
                         groups > 1 ? base : nullptr, s, kvh, row0, bits, fsh);
       if (groups > 1) {
-        __threadfence();
         __syncthreads();
         if (t == 0) {
+          __threadfence();
           const bool last = atomicAdd(all_count, 1u) == (unsigned)groups - 1;
+          __threadfence();
           if (last) *all_count = 0;
           sum_sh[2] = last;
         }
         __syncthreads();
         if (sum_sh[2]) {
-          __threadfence();
           join_partials<HD>(a, a.part + (long long)slot_of(c_first) * PART, a.part + (long long)slot_of(c_first + kJoin) * PART,
                             2ll * kJoin * PART, groups, ROWS, nullptr, s, kvh, row0, bits, fsh);
         }
@@ -830,7 +852,9 @@ static_assert(4 * 148 * 4 <= kPagedCounters, "two counters a partial, two partia
 static void plan_decode(PagedAttn &a) {
   const int rt = decode_rt(a), rows = 8 * rt;
   a.row_groups = (int)(((long long)a.max_q * a.group + rows - 1) / rows);
-  a.split_tiles = 2 * kDecWarps / rt;
+  a.split_tiles = SPLIT_T * kDecWarps / rt;
+  // (One context alone: no share holds a second beginning.)
+  a.begin_tiles = (long long)a.batch * a.pool.kv_heads * a.row_groups == 1 ? 1 : BEGIN_T;
 }
 
 size_t paged_attention_partials(const PagedAttn &args) {

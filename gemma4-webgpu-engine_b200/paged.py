@@ -20,6 +20,7 @@ _PAGE_TYPES = {"bf16": torch.bfloat16, "int8": torch.int8, "e4m3": torch.float8_
 
 BAD_PAGE, BAD_LENGTH, TIMEOUT = 1, 2, 4
 
+_I32, _FLOAT = torch.int32, torch.float32
 _workspaces: dict = {}
 _needs: dict = {}
 
@@ -28,39 +29,61 @@ def _invalid(message: str):
     return _abi.G4Error(-1, message)
 
 
-def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _on(device):
+    """(its index, the current stream there, the device that was current if another has to be)."""
+    index, current = device.index, _current_device()
+    if index == current:
+        return index, _current_stream(index), None
+    torch.cuda.set_device(index)
+    return index, _current_stream(index), current
 
 
 def _type(t: torch.Tensor, what: str) -> int:
-    try:
-        return _TYPES[t.dtype]
-    except KeyError:
-        raise _invalid(f"{what} is f32 or bf16, got {t.dtype}") from None
+    kind = _TYPES.get(t.dtype)
+    if kind is None:
+        raise _invalid(f"{what} is f32 or bf16, got {t.dtype}")
+    return kind
 
 
 def _ints(t: torch.Tensor, what: str, device, n: int) -> int:
-    if t.dtype != torch.int32 or t.device != device or t.dim() != 1 or t.numel() < n or not t.is_contiguous():
+    if t.dtype is not _I32 or t.device != device or t.dim() != 1 or t.shape[0] < n or not t.is_contiguous():
         raise _invalid(f"{what} is a contiguous int32 vector of {n} or more on {device}")
     return t.data_ptr()
 
 
 def _rows(t: torch.Tensor, what: str, device, shape) -> int:
     """Stride between rows of t [n, heads, head_dim], whose rows are contiguous."""
-    if t.device != device or tuple(t.shape) != shape:
+    if t.shape != shape or t.device != device:
         raise _invalid(f"{what} is {list(shape)} on {device}, got {list(t.shape)} on {t.device}")
-    if t.numel() and (t.stride(2) != 1 or t.stride(1) != shape[2]):
+    s = t.stride()
+    if (s[2] != 1 or s[1] != shape[2]) and t.numel():
         raise _invalid(f"{what}: one token's heads are contiguous")
-    return t.stride(0) if shape[0] > 1 else shape[1] * shape[2]
+    return s[0] if shape[0] > 1 else shape[1] * shape[2]
 
 
-def _workspace(device, stream: int, need: int) -> torch.Tensor:
-    key = (device, stream)
+def _workspace(device, index: int, stream: int, need: int) -> torch.Tensor:
+    key = (index, stream)
     ws = _workspaces.get(key)
-    if ws is None or ws.numel() < need:
+    if ws is None or ws.shape[0] < need:
         ws = torch.zeros(max(need, 1 << 20), dtype=torch.uint8, device=device)
         _workspaces[key] = ws
     return ws
+
+
+def _need(key, ask) -> int:
+    need = _needs.get(key)
+    if need is None:
+        n = C.c_uint64()
+        _abi.check(ask(C.byref(n)))
+        if len(_needs) > 4096:
+            _needs.clear()
+        need = _needs[key] = n.value
+    return need
 
 
 class PagePool:
@@ -69,23 +92,25 @@ class PagePool:
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None):
-        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _FORMATS:
+        shape, device, fmt = k.shape, k.device, _FORMATS.get(k.dtype)
+        if len(shape) != 4 or shape != v.shape or k.dtype != v.dtype or fmt is None:
             raise _invalid("k and v are [n_pages, kv_heads, page_size, head_dim] of bf16, int8 or e4m3")
-        if not k.is_cuda or k.device != v.device or not k.is_contiguous() or not v.is_contiguous():
+        if not k.is_cuda or device != v.device or not k.is_contiguous() or not v.is_contiguous():
             raise _invalid("k and v are contiguous on one CUDA device")
-        fmt = _FORMATS[k.dtype]
+        ks = vs = None
         if fmt:
             for s in (k_scale, v_scale):
-                if s is None or s.dtype != torch.float32 or s.shape != k.shape[:3] or s.device != k.device \
+                if s is None or s.dtype is not _FLOAT or s.shape != shape[:3] or s.device != device \
                         or not s.is_contiguous():
                     raise _invalid("8-bit pages need f32 scales [n_pages, kv_heads, page_size]")
+            ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
         elif k_scale is not None or v_scale is not None:
             raise _invalid("bf16 pages have no scales")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.device = k.device
-        self.n_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
-        self.struct = _abi.PagePool(k.data_ptr(), v.data_ptr(), _abi.ptr(k_scale), _abi.ptr(v_scale),
-                                    self.n_pages, self.page_size, self.kv_heads, self.head_dim, fmt)
+        self.device = device
+        self.n_pages, self.kv_heads, self.page_size, self.head_dim = shape
+        self.format = fmt
+        self.struct = _abi.PagePool(k.data_ptr(), v.data_ptr(), ks, vs, *(shape[i] for i in (0, 2, 1, 3)), fmt)
         self.ref = C.byref(self.struct)
         self.lib = _abi.load()
 
@@ -106,35 +131,36 @@ class PagePool:
 
     def store(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Quantise rows k, v [tokens, kv_heads, head_dim] into the pages at `slots`."""
-        n = k.shape[0]
+        n, device = k.shape[0], self.device
         shape = (n, self.kv_heads, self.head_dim)
-        ks, vs = _rows(k, "k", self.device, shape), _rows(v, "v", self.device, shape)
-        if k.dtype != v.dtype:
+        ks, vs = _rows(k, "k", device, shape), _rows(v, "v", device, shape)
+        if k.dtype is not v.dtype:
             raise _invalid("k and v have one type")
-        if n == 0:
-            return
-        with torch.cuda.device(self.device):
-            _abi.check(self.lib.g4_op_page_store(
-                self.ref, k.data_ptr(), v.data_ptr(), _type(k, "k"), ks, vs, n,
-                _ints(slots, "slots", self.device, n), _stream(k)))
+        kind, at = _type(k, "k"), _ints(slots, "slots", device, n)
+        _, stream, back = _on(device)
+        rc = self.lib.g4_op_page_store(self.ref, k.data_ptr(), v.data_ptr(), kind, ks, vs, n, at, stream) if n else 0
+        if back is not None:
+            torch.cuda.set_device(back)
+        _abi.check(rc)
 
     def read(self, slots: torch.Tensor, dtype=torch.float32, k_out: torch.Tensor | None = None,
              v_out: torch.Tensor | None = None):
         """The rows at `slots`, dequantised: (k, v) [tokens, kv_heads, head_dim]."""
-        n = slots.numel()
+        n, device = slots.numel(), self.device
         shape = (n, self.kv_heads, self.head_dim)
         if k_out is None:
-            k_out = torch.empty(shape, dtype=dtype, device=self.device)
+            k_out = torch.empty(shape, dtype=dtype, device=device)
         if v_out is None:
-            v_out = torch.empty(shape, dtype=dtype, device=self.device)
-        if k_out.dtype != v_out.dtype:
+            v_out = torch.empty(shape, dtype=dtype, device=device)
+        if k_out.dtype is not v_out.dtype:
             raise _invalid("k_out and v_out have one type")
-        ks, vs = _rows(k_out, "k_out", self.device, shape), _rows(v_out, "v_out", self.device, shape)
-        if n:
-            with torch.cuda.device(self.device):
-                _abi.check(self.lib.g4_op_page_read(
-                    self.ref, _ints(slots, "slots", self.device, n), n, _type(k_out, "dtype"),
-                    k_out.data_ptr(), v_out.data_ptr(), ks, vs, _stream(k_out)))
+        ks, vs = _rows(k_out, "k_out", device, shape), _rows(v_out, "v_out", device, shape)
+        kind, at = _type(k_out, "dtype"), _ints(slots, "slots", device, n)
+        _, stream, back = _on(device)
+        rc = self.lib.g4_op_page_read(self.ref, at, n, kind, k_out.data_ptr(), v_out.data_ptr(), ks, vs, stream) if n else 0
+        if back is not None:
+            torch.cuda.set_device(back)
+        _abi.check(rc)
         return k_out, v_out
 
 
@@ -148,44 +174,48 @@ def attention(pool: PagePool, q: torch.Tensor, q_begin: torch.Tensor, q_pos: tor
     dev = pool.device
     if q.dim() != 3:
         raise _invalid("q is [rows, heads, head_dim]")
-    rows, heads = q.shape[0], q.shape[1]
+    rows, heads, _ = q.shape
     shape = (rows, heads, pool.head_dim)
     qs = _rows(q, "q", dev, shape)
     kind = _type(q, "q")
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=dev)
-    elif out.dtype != q.dtype:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        os = heads * pool.head_dim
+    elif out.dtype is not q.dtype:
         raise _invalid("out has q's type")
-    os = _rows(out, "out", dev, shape)
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != dev \
-            or (page_table.numel() and page_table.stride(1) != 1):
+    else:
+        os = _rows(out, "out", dev, shape)
+    if page_table.dim() != 2 or page_table.dtype is not _I32 or page_table.device != dev:
         raise _invalid(f"page_table is int32 [batch, pages] on {dev}")
     batch, width = page_table.shape
-    if lse is not None and (lse.dtype != torch.float32 or lse.device != dev or not lse.is_contiguous()
-                            or tuple(lse.shape) != (rows, heads)):
+    stride, step = page_table.stride()
+    if batch < 2:
+        stride = width
+    if (step != 1 and width > 1) or stride < width:
+        raise _invalid("page_table's rows are contiguous and do not overlap")
+    if lse is not None and (lse.dtype is not _FLOAT or lse.device != dev or not lse.is_contiguous()
+                            or lse.shape != (rows, heads)):
         raise _invalid("lse is f32 [rows, heads]")
-    stride = page_table.stride(0) if batch > 1 else width
-    if stride < width:
-        raise _invalid("page_table's rows overlap")
-    stream = _stream(q)
-    with torch.cuda.device(dev):
-        key = (pool.kv_heads, pool.page_size, pool.head_dim, pool.struct.format, kind, heads, rows,
-               batch, max_q, max_kv, window)
-        need = _needs.get(key)
-        if need is None:
-            n = C.c_uint64()
-            _abi.check(pool.lib.g4_op_paged_attention_workspace(
-                pool.ref, kind, heads, rows, batch, max_q, max_kv, window, C.byref(n)))
-            if len(_needs) > 4096:
-                _needs.clear()
-            need = _needs[key] = n.value
-        ws = _workspace(dev, stream, need)
-        # Positions past the table's width are cut off by the stride only when it equals the width.
-        _abi.check(pool.lib.g4_op_paged_attention(
-            pool.ref, q.data_ptr(), qs, out.data_ptr(), os, _abi.ptr(lse), kind, heads, rows, batch,
-            _ints(q_begin, "q_begin", dev, batch + 1), _ints(q_pos, "q_pos", dev, batch),
-            _ints(kv_len, "kv_len", dev, batch), page_table.data_ptr(), stride, max_q,
-            min(max_kv, width * pool.page_size), window, scale, ws.data_ptr(), ws.numel(), stream))
+    begin, pos, length = (_ints(q_begin, "q_begin", dev, batch + 1), _ints(q_pos, "q_pos", dev, batch),
+                          _ints(kv_len, "kv_len", dev, batch))
+    # Positions past the table's width are cut off, as those past max_kv are.
+    max_kv = min(max_kv, width * pool.page_size)
+    index, stream, back = _on(dev)
+    try:
+        lib = pool.lib
+        need = _need((pool.kv_heads, pool.page_size, pool.head_dim, pool.format, kind, heads, rows, batch, max_q, max_kv,
+                      window), lambda n: lib.g4_op_paged_attention_workspace(
+                          pool.ref, kind, heads, rows, batch, max_q, max_kv, window, n))
+        ws = _workspace(dev, index, stream, need)
+        rc = lib.g4_op_paged_attention(
+            pool.ref, q.data_ptr(), qs, out.data_ptr(), os, None if lse is None else lse.data_ptr(), kind, heads, rows,
+            batch, begin, pos, length, page_table.data_ptr(), stride, max_q, max_kv, window, scale, ws.data_ptr(),
+            ws.shape[0], stream)
+    finally:
+        if back is not None:
+            torch.cuda.set_device(back)
+    if rc:
+        _abi.check(rc)
     return out
 
 
@@ -198,37 +228,38 @@ def verify_drafts(logits: torch.Tensor, row_begin: torch.Tensor, drafts: torch.T
     if logits.dim() != 2 or not logits.is_cuda or logits.stride(1) != 1:
         raise _invalid("logits is [rows, vocab] on a CUDA device, rows contiguous")
     rows, vocab = logits.shape
-    batch = row_begin.numel() - 1
+    batch = row_begin.shape[0] - 1
     kind = _type(logits, "logits")
     for t, what, n in ((uniforms, "uniforms", rows), (temperature, "temperature", batch)):
-        if t.dtype != torch.float32 or t.device != dev or t.numel() < n or not t.is_contiguous():
+        if t.dtype is not _FLOAT or t.device != dev or t.numel() < n or not t.is_contiguous():
             raise _invalid(f"{what} is a contiguous f32 vector of {n} or more on {dev}")
     for t, what, n in ((gumbel, "gumbel", batch), (draft_probs, "draft_probs", rows)):
-        if t is not None and (t.dtype != torch.float32 or t.device != dev or t.dim() != 2
+        if t is not None and (t.dtype is not _FLOAT or t.device != dev or t.dim() != 2
                               or t.shape[0] < n or t.shape[1] != vocab or t.stride(1) != 1):
             raise _invalid(f"{what} is f32 [{n}, {vocab}] on {dev}, rows contiguous")
+    begin, at = _ints(row_begin, "row_begin", dev, batch + 1), _ints(drafts, "drafts", dev, rows)
+    if max_drafts < 0 or batch < 0:
+        raise _invalid("max_drafts is not negative, and row_begin holds one more than the sequences")
     lib = _abi.load()
-    tokens = torch.empty((batch, max_drafts + 1), dtype=torch.int32, device=dev)
-    logprobs = torch.empty((batch, max_drafts + 1), dtype=torch.float32, device=dev)
-    counts = torch.empty(batch, dtype=torch.int32, device=dev)
-    stream = _stream(logits)
-    with torch.cuda.device(dev):
-        key = (vocab, rows, batch, max_drafts)
-        need = _needs.get(key)
-        if need is None:
-            n = C.c_uint64()
-            _abi.check(lib.g4_op_verify_drafts_workspace(vocab, rows, batch, max_drafts, C.byref(n)))
-            if len(_needs) > 4096:
-                _needs.clear()
-            need = _needs[key] = n.value
-        ws = _workspace(dev, stream, need)
-        _abi.check(lib.g4_op_verify_drafts(
-            logits.data_ptr(), logits.stride(0), kind, vocab, rows, batch,
-            _ints(row_begin, "row_begin", dev, batch + 1), _ints(drafts, "drafts", dev, rows),
-            _abi.ptr(draft_probs), 0 if draft_probs is None else draft_probs.stride(0),
-            uniforms.data_ptr(), gumbel.data_ptr(), gumbel.stride(0), temperature.data_ptr(),
-            max_drafts, tokens.data_ptr(), logprobs.data_ptr(), counts.data_ptr(), ws.data_ptr(),
-            ws.numel(), stream))
+    tokens = torch.empty((batch, max_drafts + 1), dtype=_I32, device=dev)
+    logprobs = torch.empty((batch, max_drafts + 1), dtype=_FLOAT, device=dev)
+    counts = torch.empty(batch, dtype=_I32, device=dev)
+    index, stream, back = _on(dev)
+    try:
+        need = _need((vocab, rows, batch, max_drafts), lambda n: lib.g4_op_verify_drafts_workspace(
+            vocab, rows, batch, max_drafts, n))
+        ws = _workspace(dev, index, stream, need)
+        rc = lib.g4_op_verify_drafts(
+            logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, kind, vocab, rows, batch, begin, at,
+            None if draft_probs is None else draft_probs.data_ptr(),
+            0 if draft_probs is None else draft_probs.stride(0) if rows > 1 else vocab, uniforms.data_ptr(),
+            gumbel.data_ptr(), gumbel.stride(0) if batch > 1 else vocab, temperature.data_ptr(), max_drafts,
+            tokens.data_ptr(), logprobs.data_ptr(), counts.data_ptr(), ws.data_ptr(), ws.shape[0], stream)
+    finally:
+        if back is not None:
+            torch.cuda.set_device(back)
+    if rc:
+        _abi.check(rc)
     return tokens, logprobs, counts
 
 

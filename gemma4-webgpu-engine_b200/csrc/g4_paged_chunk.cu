@@ -20,8 +20,10 @@
 //  - One thread issues the products in the order S(j), O(j - 1), so the softmax of block j runs
 //    under the products of its neighbours.
 //  - Softmax: two threads a row, 64 positions of a block each, held in registers from the scores to
-//    the weights. The maximum is stale by up to a factor of 2^1.9 (weights stay
-//    below f16's greatest number); only when a row outgrows it are its warp's O rows rescaled.
+//    the weights. The maximum is stale by up to a factor of 2^2.9; only when a row outgrows it are its
+//    warp's O rows rescaled (1,000 to 4,000 cycles). Weights are scaled by 2^13, so they stay below
+//    f16's greatest number and are held to 2^-38 of the row's greatest; a staler maximum would cost
+//    that.
 // head_dim 512: O would fill tensor memory alone, so two blocks compute the scores each and take
 // half of V's dimensions (1.5 times the operations).
 #include <cuda_runtime.h>
@@ -188,7 +190,11 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
   return r;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 template <bool HALF>
 __device__ __forceinline__ uint32_t pack16(float a, float b) {
@@ -650,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
   }
   float m = -INFINITY, l = 0.0f;
   int lo = 0, hi = 0;
-  const float bits = HALF ? 14.0f : 0.0f;
+  const float bits = HALF ? 13.0f : 0.0f;
   const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
   const int row = 32 * (warp & 3) + lane, ch = (warp >> 2) & 1;   // softmax: thread's row, its half of the columns
   if (warp < kSoftWarps) {
@@ -662,7 +668,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
     for (int j = 0; j < nb; j++) {
       const int k = j % NSC, pos0 = (j0 + j) * BN + 64 * ch;
       const auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory"); };
-      ok = ok && warp_wait(&info_full[k], (uint32_t)((j / NSC) & 1)) && warp_wait(&s_full[j & 1], (uint32_t)((j >> 1) & 1));
+      if (ok) {
+        const uint32_t pi = (uint32_t)((j / NSC) & 1), ps = (uint32_t)((j >> 1) & 1);
+        ok = __all_sync(0xffffffffu, mbar_try_wait(&info_full[k], pi) && mbar_try_wait(&s_full[j & 1], ps)) ||
+             (warp_wait(&info_full[k], pi) && warp_wait(&s_full[j & 1], ps));
+      }
       if (!ok) {   // the other half's warp still counts on this one's barriers
         pair_sync();
         continue;
@@ -679,6 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
       // The scores in units of log2, less the row's factor in the plain case.
       float top = -INFINITY;
       if (plain) {
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
@@ -692,10 +703,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
               z[h][i + 2] = w.x;
               z[h][i + 3] = w.y;
             }
-            top = max3(top, z[h][i], z[h][i + 1]);
-            top = max3(top, z[h][i + 2], z[h][i + 3]);
+            tops[0 + (i & 4) / 2] = max3(tops[0 + (i & 4) / 2], z[h][i], z[h][i + 1]);
+            tops[1 + (i & 4) / 2] = max3(tops[1 + (i & 4) / 2], z[h][i + 2], z[h][i + 3]);
           }
-        top = top * qf + (HALF ? f.lmax : 0.0f);
+        top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * qf + (HALF ? f.lmax : 0.0f);
       } else {
 #pragma unroll
         for (int h = 0; h < 2; h++)
@@ -711,8 +722,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
       row_top[j & 1][ch][row] = top;
       pair_sync();
       top = fmaxf(top, row_top[j & 1][ch ^ 1][row]);
-      // The maximum moves only when a row outgrows it by more than 2^1.9.
-      const bool grow = top > m + 1.9f;
+      // The maximum moves only when a row outgrows it by more than 2^2.9.
+      const bool grow = top > m + 2.9f;
       if (__any_sync(0xffffffffu, grow)) {
         const float e = grow ? cex2(m - top) : 1.0f;
         if (grow) {
@@ -736,7 +747,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
         }
       }
       const float r = m == -INFINITY ? 0.0f : m - bits;
-      F2 sum = f2(0.0f, 0.0f);
+      F2 sum = f2(0.0f, 0.0f), sum1 = sum;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         uint32_t pk[16];
@@ -747,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
             const float2 y0 = un2(fma2(f2(z[h][i], z[h][i + 1]), q2, r2)), y1 = un2(fma2(f2(z[h][i + 2], z[h][i + 3]), q2, r2));
             F2 p0 = f2(cex2(y0.x), cex2(y0.y)), p1 = f2(cex2(y1.x), cex2(y1.y));
             sum = add2(sum, p0);
-            sum = add2(sum, p1);
+            sum1 = add2(sum1, p1);
             if (HALF) {
               const float4 c = vs[8 * h + i / 4];
               p0 = mul2(p0, f2(c.x, c.y));
@@ -768,7 +779,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
         }
         tst16(at + 16 * h, pk);
       }
-      const float2 two = un2(sum);
+      const float2 two = un2(add2(sum, sum1));
       l += two.x + two.y;
       tst_wait();
       fence_before();

@@ -15,7 +15,7 @@
 //    product of N 64 costs 112 cycles, not the 32 of its share (head_dim 256 by columns took 3,600
 //    cycles a block for O, 8 products of N 256 are 1,024). Both are written alike. Six producer warps gather the
 //    pages' rows, each a slot of its own: 8-bit codes through registers, the next slot's requested
-//    as this one's are widened to f16, bf16 rows by asynchronous copies. A scout warp reads the
+//    as this one's are widened to f16, bf16 rows by TMA. A scout warp reads the
 //    page table and the scales blocks ahead.
 //  - One thread issues the products in the order S(j), O(j - 1), so the softmax of block j runs
 //    under the products of its neighbours.
@@ -106,6 +106,14 @@ __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::be
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void commit(uint64_t *bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// A copy of 16 rows of the pool, 128 bytes of each from byte x, into the 128-byte swizzle (bf16 pages).
+__device__ __forceinline__ void tma_rows(void *dst, const CUtensorMap *map, int x, int row, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(smem_u32(bar))
+      : "memory");
 }
 // Shared-memory matrix descriptor, 128-byte swizzle, 8-row groups 1024 bytes apart. It serves both
 // uses of a slot: K-major (rows are N, 64 K elements a row) and MN-major (rows are K, 64 N
@@ -249,7 +257,8 @@ struct RowTile {
 
 // Block (row tile x half of V, KV head, sequence).
 template <int FMT, int HD>
-__global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) {
+__global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a, const __grid_constant__ CUtensorMap map_k,
+                                                          const __grid_constant__ CUtensorMap map_v) {
   using S = ChunkShape<FMT, HD>;
   constexpr bool HALF = S::HALF;
   constexpr int NH = HD / S::OD;
@@ -277,6 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
   uint64_t *info_full = pv_done + 1, *info_free = info_full + NSC, *end = info_free + NSC;
   uint32_t *tslot = reinterpret_cast<uint32_t *>(end + 1);
   int *failed = reinterpret_cast<int *>(tslot + 1);
+  __shared__ uint64_t own_bar[S::PW];
   __shared__ uint32_t bad_v[4][4];   // bf16 pages: positions of boundary blocks whose V is not finite
   __shared__ float q_scale[128], row_top[2][2][128];
   auto slot = [&](int i) { return csm + S::Q_BYTES + i * SLOT; };
@@ -297,6 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
       mbar_init(&info_free[i], kSoftWarps + S::VC);
     }
     mbar_init(end, 1);
+    for (int i = 0; i < S::PW; i++) mbar_init(&own_bar[i], 1);
     mbar_fence_init();
     *failed = 0;
   }
@@ -468,36 +479,42 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
         if (more) used(next);
       }
     } else {
-      // Piece k of a lane: 8 values of row 4 k + lane / 8 of the slot's columns laid end to end.
-      const int rr = lane >> 3, x = lane & 7;
+      // Eight copies of 16 rows x 64 dimensions, swizzled on the way, a lane each. They count on the
+      // slot's barrier; where V has to be looked over first, on the warp's own.
+      uint64_t *const own = &own_bar[w];
+      uint32_t turn = 0;
+      int asked = w;   // the slot after the last one asked for
 #pragma unroll 1
       for (int i = w; i < total; i += S::PW) {
         const SlotAt<S::KC, S::VC> at(i, nb);
         ok = known(at) && slot_free(i);
         if (!ok) break;
-        const uint8_t *base = (at.v ? p.v + half * S::OD * 2 : p.k + at.c * 128) + rr * ROW + x * 16;
-        const bool partly = odd_block(at.j);
-        const long long *rows = info[at.j % NSC].at;
-        uint8_t *to = slot(i % S::NS);
-#pragma unroll 8
-        for (int k = 0; k < 32; k++) {
-          const int r = 4 * k + rr, q = at.v ? at.c * S::TV + 4 * (k % (S::TV / 4)) + rr : r;   // q: position in the block
-          const long long row = rows[q >> 4] + (at.v ? 128 * (k / (S::TV / 4)) : 0);
-          uint8_t *dst = to + r * 128 + ((x ^ (r & 7)) << 4);
-          if (!partly || seen(at.j, q))
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(base + row + (k & 3) * 4 * ROW) : "memory");
-          else
-            *reinterpret_cast<uint4 *>(dst) = make_uint4(0, 0, 0, 0);
+        const int sl = i % S::NS;
+        const bool partly = at.v && odd_block(at.j);
+        uint64_t *const bar = partly ? own : &full[sl];
+        if (lane == 0) mbar_expect_tx(bar, SLOT);
+        __syncwarp();
+        if (lane < 8) {
+          constexpr int T = S::TV / 16;   // tiles of a V slot's column
+          const int tile = at.v ? at.c * T + lane % T : lane, col = at.v ? half * S::VC + lane / T : at.c;
+          tma_rows(slot(sl) + lane * 2048, at.v ? &map_v : &map_k, col * 128, (int)(info[at.j % NSC].at[tile] / ROW), bar);
         }
-        used(at);
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        if (at.v && edge(at.j)) {
-          // A block that some row sees only in part: a weight of 0 must not meet an infinity or a NaN.
+        asked = i + S::PW;
+        if (partly) {
+          ok = warp_wait(own, turn);
+          turn ^= 1;
+          if (!ok) break;
+          // A weight of 0 must not meet an infinity or a NaN: positions no row sees become 0, and so do
+          // values that are not finite in a block that some row sees only in part (rows that see them
+          // are told by bad_v).
+          const int rr = lane >> 3, x = lane & 7;
+          const bool cut = edge(at.j);
 #pragma unroll 1
           for (int k = 0; k < 32; k++) {
             const int r = 4 * k + rr, pos = at.c * S::TV + 4 * (k % (S::TV / 4)) + rr;
-            uint4 *q = reinterpret_cast<uint4 *>(to + r * 128 + ((x ^ (r & 7)) << 4));
+            uint4 *q = reinterpret_cast<uint4 *>(slot(sl) + r * 128 + ((x ^ (r & 7)) << 4));
             uint32_t u[4] = {q->x, q->y, q->z, q->w};
+            const bool gone = !seen(at.j, pos);
             bool bad = false;
 #pragma unroll
             for (int z = 0; z < 4; z++) {
@@ -510,17 +527,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_chunk(const PagedAttn a) 
                 bad = true;
               }
             }
-            if (bad) {
+            if (gone)
+              *q = make_uint4(0, 0, 0, 0);
+            else if (bad && cut) {
               *q = make_uint4(u[0], u[1], u[2], u[3]);
               atomicOr(&bad_v[at.j < 2 ? at.j : 2 + (nb - 1 - at.j)][pos >> 5], 1u << (pos & 31));
             }
           }
+          fence_async();
+          __syncwarp();
+          if (lane == 0) arrive(&full[sl]);
         }
-        fence_async();
-        __syncwarp();
-        if (lane == 0) arrive(&full[i % S::NS]);
+        used(at);
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");
+      // Every copy asked for has landed before the block can end: those of the ring's last round are
+      // waited for here (a slot filled again since is of a round that its barrier no longer tells).
+      for (int i = asked - S::PW; i >= w && i >= total - S::NS; i -= S::PW) warp_wait(&full[i % S::NS], (uint32_t)((i / S::NS) & 1));
     }
     if (!ok) {
       *failed = 1;
@@ -861,7 +883,15 @@ static cudaError_t launch_chunk_hd(const PagedAttn &a, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   const int tpt = 128 / a.group, tiles = (a.max_q + tpt - 1) / tpt;
   const dim3 grid((unsigned)(tiles * (HD / S::OD)), a.pool.kv_heads, a.batch);
-  return launch_k(k_paged_chunk<FMT, HD>, grid, dim3(kThreads), S::SMEM, st, false, a);
+  CUtensorMap map_k = {}, map_v = {};
+  if (!S::HALF) {
+    // Rows of the pool as bytes; head_dim 64 or more of them stay far below 2^31.
+    const uint64_t rows = (uint64_t)a.pool.n_pages * a.pool.kv_heads * a.pool.page_size;
+    if (rows >= 1ull << 31 || make_tmap_u8(&map_k, a.pool.k, 2 * HD, rows, 2 * HD, 128, 16, true) ||
+        make_tmap_u8(&map_v, a.pool.v, 2 * HD, rows, 2 * HD, 128, 16, true))
+      return cudaErrorInvalidValue;
+  }
+  return launch_k(k_paged_chunk<FMT, HD>, grid, dim3(kThreads), S::SMEM, st, false, a, map_k, map_v);
 }
 template <int FMT>
 static cudaError_t launch_chunk(const PagedAttn &a, cudaStream_t st) {

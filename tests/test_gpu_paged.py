@@ -604,3 +604,60 @@ def test_sampling_follows_the_target(paged, cuda):
                                            draft_probs=qp.expand(2 * B, V).contiguous() if probs else None)
         f = torch.bincount(tokens[:, 0].long(), minlength=V).double() / B
         assert ((f - p).abs() <= 5 * (p * (1 - p) / B).sqrt() + 1e-12).all(), (probs, f.tolist(), p.tolist())
+
+
+# ------------------------------------------------------------------------------ together
+
+@pytest.mark.parametrize("fmt,window", [("int8", 0), ("e4m3", 24), ("bf16", 0)])
+def test_example_speculation_gives_the_plain_greedy_tokens(paged, cuda, fmt, window):
+    """The example's server: with drafts, in fewer passes, the tokens that one at a time gives."""
+    example = importlib.import_module("examples.paged_speculation")
+    out = example.main(["--tokens", "40", "--format", fmt, "--window", str(window)])
+    assert out["ids"] == out["plain"] and all(len(x) == 40 for x in out["ids"])
+    assert out["plain_passes"] == 40 and out["passes"] < 40 and out["accepted"] > 0
+
+
+def test_example_samples_at_a_temperature(paged, cuda):
+    example = importlib.import_module("examples.paged_speculation")
+    out = example.main(["--tokens", "12", "--temperature", "0.9"])
+    assert all(len(x) == 12 and all(0 <= t < 384 for t in x) for x in out["ids"])
+
+
+@pytest.mark.parametrize("q_len", [1, 40])
+@pytest.mark.parametrize("window", [0, 40])
+def test_e4m3_positions_that_no_row_sees_may_hold_nan_codes(paged, cuda, q_len, window):
+    """Memory of a page that was never written, or that belongs to positions below the window."""
+    torch = cuda
+    kv = 150
+    table, pages = layout(torch, [kv], 64, 1, 4)
+    pool = make_pool(paged, torch, "e4m3", pages, 64, 1, 128, 4)
+    pos = kv - q_len
+    lo = max(0, pos - window + 1) if window else 0
+    for x in (pool.k, pool.v):
+        raw = x.view(torch.uint8)
+        for t in list(range(0, lo)) + list(range(kv, 3 * 64)):
+            raw[int(table[0, t // 64]), :, t % 64] = 0x7F
+    q = torch.randn(q_len, 8, 128, generator=gen(torch, 9), device="cuda").bfloat16()
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    out = paged.attention(pool, q, ints([0, q_len]), ints([pos]), ints([kv]), table, q_len, kv, window=window, scale=0.05)
+    want = reference(torch, pool, q, [(0, q_len, pos, kv)], table, window, float(np.float32(0.05)))
+    check(torch, out, None, *want, True)
+
+
+@pytest.mark.parametrize("q_len", [2, 40])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_bf16_values_a_row_does_not_see_never_reach_it(paged, cuda, q_len, bad):
+    """One new token's V holds a value that is not finite: the rows before it stay finite and right, those
+    from it on are not finite where the value enters."""
+    torch = cuda
+    kv = 100
+    table, pages = layout(torch, [kv], 16, 1, 4)
+    pool = make_pool(paged, torch, "bf16", pages, 16, 1, 128, 4)
+    q = torch.randn(q_len, 8, 128, generator=gen(torch, 9), device="cuda").bfloat16()
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    args = (ints([0, q_len]), ints([kv - q_len]), ints([kv]), table, q_len, kv)
+    good = paged.attention(pool, q, *args, scale=0.05)
+    pool.v[int(table[0, (kv - 1) // 16]), 0, (kv - 1) % 16, 5] = bad
+    out = paged.attention(pool, q, *args, scale=0.05)
+    assert torch.equal(out[:-1], good[:-1])
+    assert not out[-1, :, 5].isfinite().any()

@@ -85,14 +85,17 @@ __device__ __forceinline__ float logit_at(const DraftArgs &a, long long row, int
     return __bfloat162float(*p);
 }
 
-// VEC consecutive elements at p (aligned to VEC elements).
-template <typename T, int VEC>
-__device__ __forceinline__ void load_vec(const T *p, float (&x)[VEC]) {
-  if constexpr (VEC == 1) {
-    if constexpr (sizeof(T) == 4)
-      x[0] = __ldg(p);
-    else
-      x[0] = __bfloat162float(*p);
+// Four consecutive elements at p: one load where p is aligned to them, else four.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load4(const T *p, float (&x)[4]) {
+  if constexpr (!WIDE) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      if constexpr (sizeof(T) == 4)
+        x[e] = __ldg(p + e);
+      else
+        x[e] = __bfloat162float(p[e]);
+    }
   } else if constexpr (sizeof(T) == 4) {
     const float4 v = __ldg(reinterpret_cast<const float4 *>(p));
     x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
@@ -103,6 +106,11 @@ __device__ __forceinline__ void load_vec(const T *p, float (&x)[VEC]) {
     x[2] = __uint_as_float(v.y << 16);
     x[3] = __uint_as_float(v.y & 0xffff0000u);
   }
+}
+// Elements before the first one that is aligned to four.
+template <typename T>
+__device__ __forceinline__ int before4(const T *p) {
+  return (int)((-(intptr_t)p & (4 * sizeof(T) - 1)) / sizeof(T));
 }
 
 struct SeqRows {
@@ -126,8 +134,9 @@ struct DraftState {
 };
 
 // Block (split, j, b): split's share of sequence b's row j. The sequence's last block to finish
-// joins the shares and decides.
-template <typename T, int VEC>
+// joins the shares and decides. Shares begin where the row's logits are aligned to four, so these always
+// come four a load; NW: so does the noise.
+template <typename T, bool NW>
 __global__ void __launch_bounds__(kDraftThreads) k_draft_scan(const DraftArgs a, DraftState *state) {
   const int b = blockIdx.z, j = blockIdx.y, split = blockIdx.x, t = threadIdx.x;
   const SeqRows sr = seq_rows(a, b, j == 0 && split == 0 && t == 0);
@@ -160,21 +169,22 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_scan(const DraftArgs a,
   const float *noise = a.gumbel + (long long)b * a.ld_gumbel;
   RowSum sum{-INFINITY, 0.0f};
   Race best{-INFINITY, 0x7fffffff};
-  const int c0 = split * a.chunk, c1 = min(a.vocab, c0 + a.chunk);
-  constexpr int U = 16 / VEC, STEP = kDraftThreads * VEC;   // loads in flight of each kind
+  const int head = before4(src);   // tokens before the first share's first load
+  const int c0 = split * a.chunk + head, c1 = min(a.vocab, c0 + a.chunk);
+  constexpr int U = 4, STEP = kDraftThreads * 4;   // loads in flight of each kind
   // One pass of 16 tokens a thread. FULL: all of them are there and none is left out.
   auto pass = [&](auto full_, auto race_, auto noisy_, int i0) {
     constexpr bool FULL = decltype(full_)::value, RACE = decltype(race_)::value, NOISY = decltype(noisy_)::value;
-    float x[U][VEC], g[U][VEC];
+    float x[U][4], g[U][4];
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const int i = i0 + u * STEP;
-      if (FULL || i + VEC <= c1) {
-        load_vec<T, VEC>(src + i, x[u]);
-        if (NOISY) load_vec<float, VEC>(noise + i, g[u]);
+      if (FULL || i + 4 <= c1) {
+        load4<T, true>(src + i, x[u]);
+        if (NOISY) load4<float, NW>(noise + i, g[u]);
       } else {
 #pragma unroll
-        for (int e = 0; e < VEC; e++) {
+        for (int e = 0; e < 4; e++) {
           x[u][e] = i + e < c1 ? logit_at<T>(a, row, i + e) : -INFINITY;
           g[u][e] = NOISY && i + e < c1 ? noise[i + e] : 0.0f;
         }
@@ -184,7 +194,7 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_scan(const DraftArgs a,
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
-      for (int e = 0; e < VEC; e++) {
+      for (int e = 0; e < 4; e++) {
         x[u][e] = __fmul_rn(x[u][e], inv);
         top = fmaxf(top, x[u][e]);
       }
@@ -193,8 +203,8 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_scan(const DraftArgs a,
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
-      for (int e = 0; e < VEC; e++) {
-        ((u * VEC + e) & 1 ? s1 : s0) += ex2(fmaf(x[u][e], kLog2e, low));
+      for (int e = 0; e < 4; e++) {
+        (e & 1 ? s1 : s0) += ex2(fmaf(x[u][e], kLog2e, low));
         if (RACE) {
           const int i = i0 + u * STEP + e;
           const float key = NOISY ? __fadd_rn(x[u][e], g[u][e]) : x[u][e];
@@ -204,8 +214,15 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_scan(const DraftArgs a,
     sum = {top, s0 + s1};
   };
   auto passes = [&](auto race_, auto noisy_) {
+    if (split == 0 && t < head && t < a.vocab) {
+      const float x = __fmul_rn(logit_at<T>(a, row, t), inv);
+      const float key = decltype(noisy_)::value ? __fadd_rn(x, noise[t]) : x;
+      // (A NaN makes the row's sum one, as in the passes.)
+      sum = {fmaxf(x, -INFINITY), x == -INFINITY ? 0.0f : ex2(fmaf(x, kLog2e, -x * kLog2e))};
+      if (decltype(race_)::value && key > best.key && t != left_out) best = {key, t};
+    }
     for (int b0 = c0; b0 < c1; b0 += STEP * U) {
-      const int i0 = b0 + t * VEC;
+      const int i0 = b0 + t * 4;
       if (b0 + STEP * U <= c1 && (left_out < b0 || left_out >= b0 + STEP * U))
         pass(std::true_type{}, race_, noisy_, i0);
       else
@@ -291,7 +308,7 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_scan(const DraftArgs a,
 
 // The remainder's race over the refused row of each sequence whose drafter gave probabilities:
 // ln max(p - q, 0) + gumbel, and x + gumbel for the case that no remainder is left.
-template <typename T, int VEC>
+template <typename T, bool NW>
 __global__ void __launch_bounds__(kDraftThreads) k_draft_rest(const DraftArgs a, const DraftState *state) {
   const int b = blockIdx.y, split = blockIdx.x, t = threadIdx.x;
   const DraftState st = state[b];
@@ -304,20 +321,31 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_rest(const DraftArgs a,
   const float *probs = a.probs + (long long)st.row * a.ld_probs;
   // `s` and `m` carry the plain race here: its key, and its token as a float's bits.
   Race rest{-INFINITY, 0x7fffffff}, plain{-INFINITY, 0x7fffffff};
-  const int c1 = min(a.vocab, (split + 1) * a.chunk);
-  constexpr int U = 8 / VEC;
-  for (int i0 = split * a.chunk + t * VEC; i0 < c1; i0 += kDraftThreads * VEC * U) {
-    float x[U][VEC], g[U][VEC], q[U][VEC];
+  const int head = before4(src), c0 = split * a.chunk + head, c1 = min(a.vocab, c0 + a.chunk);
+  auto race = [&](int i, float x, float g, float q) {
+    const float xs = __fmul_rn(x, inv);
+    const float left = __fsub_rn(expf(__fsub_rn(xs, st.lse)), q);
+    if (left > 0.0f) {
+      const float key = __fadd_rn(logf(left), g);
+      if (key > rest.key) rest = {key, i};
+    }
+    const float key = __fadd_rn(xs, g);
+    if (key > plain.key) plain = {key, i};
+  };
+  if (split == 0 && t < head && t < a.vocab) race(t, logit_at<T>(a, st.row, t), noise[t], probs[t]);
+  constexpr int U = 2, STEP = kDraftThreads * 4;
+  for (int i0 = c0 + t * 4; i0 < c1; i0 += STEP * U) {
+    float x[U][4], g[U][4], q[U][4];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int i = i0 + u * kDraftThreads * VEC;
-      if (i + VEC <= c1) {
-        load_vec<T, VEC>(src + i, x[u]);
-        load_vec<float, VEC>(noise + i, g[u]);
-        load_vec<float, VEC>(probs + i, q[u]);
+      const int i = i0 + u * STEP;
+      if (i + 4 <= c1) {
+        load4<T, true>(src + i, x[u]);
+        load4<float, NW>(noise + i, g[u]);
+        load4<float, NW>(probs + i, q[u]);
       } else {
 #pragma unroll
-        for (int e = 0; e < VEC; e++) {
+        for (int e = 0; e < 4; e++) {
           const bool in = i + e < c1;
           x[u][e] = in ? logit_at<T>(a, st.row, i + e) : -INFINITY;
           g[u][e] = in ? noise[i + e] : 0.0f;
@@ -328,17 +356,7 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_rest(const DraftArgs a,
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
-      for (int e = 0; e < VEC; e++) {
-        const int i = i0 + u * kDraftThreads * VEC + e;
-        const float xs = __fmul_rn(x[u][e], inv);
-        const float left = __fsub_rn(expf(__fsub_rn(xs, st.lse)), q[u][e]);
-        if (left > 0.0f) {
-          const float key = __fadd_rn(logf(left), g[u][e]);
-          if (key > rest.key) rest = {key, i};
-        }
-        const float key = __fadd_rn(xs, g[u][e]);
-        if (key > plain.key) plain = {key, i};
-      }
+      for (int e = 0; e < 4; e++) race(i0 + u * STEP + e, x[u][e], g[u][e], q[u][e]);
   }
   const DraftPart r = block_join({-INFINITY, 0.0f, rest.key, rest.idx}, sh);
   __syncthreads();
@@ -375,13 +393,13 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_rest(const DraftArgs a,
   }
 }
 
-// Tokens a block scans: 16384, or fewer (in steps of 2048) until the rows fill the SMs twice.
+// Tokens a block scans: 16384, or fewer (in steps of 1024) until the rows fill the SMs twice.
 static int draft_chunk(int vocab, int rows) {
   const int want = 2 * 148 / (rows > 0 ? rows : 1);
   int splits = (vocab + 16383) / 16384;
   if (splits < want) splits = want;
-  int chunk = (vocab + splits - 1) / splits;
-  return (chunk + 2047) / 2048 * 2048;
+  const int chunk = (vocab + splits - 1) / splits;
+  return (chunk + 1023) / 1024 * 1024;
 }
 
 size_t verify_drafts_partials(int vocab, int rows, int batch, int max_drafts) {
@@ -389,11 +407,11 @@ size_t verify_drafts_partials(int vocab, int rows, int batch, int max_drafts) {
   return (size_t)batch * (max_drafts + 1) * splits * sizeof(DraftPart) + (size_t)batch * sizeof(DraftState);
 }
 
-template <typename T, int VEC>
+template <typename T, bool NW>
 static cudaError_t launch_drafts(const DraftArgs &a, DraftState *state, cudaStream_t st) {
   const dim3 block(kDraftThreads);
-  cudaError_t e = launch_k(k_draft_scan<T, VEC>, dim3(a.splits, a.max_drafts + 1, a.batch), block, 0, st, false, a, state);
-  if (e == cudaSuccess && a.probs) e = launch_k(k_draft_rest<T, VEC>, dim3(a.splits, a.batch), block, 0, st, false, a, state);
+  cudaError_t e = launch_k(k_draft_scan<T, NW>, dim3(a.splits, a.max_drafts + 1, a.batch), block, 0, st, false, a, state);
+  if (e == cudaSuccess && a.probs) e = launch_k(k_draft_rest<T, NW>, dim3(a.splits, a.batch), block, 0, st, false, a, state);
   return e;
 }
 
@@ -402,12 +420,13 @@ cudaError_t launch_verify_drafts(const DraftArgs &args, cudaStream_t st) {
   a.chunk = draft_chunk(a.vocab, a.rows);
   a.splits = (a.vocab + a.chunk - 1) / a.chunk;
   DraftState *state = reinterpret_cast<DraftState *>(a.part + (size_t)a.batch * (a.max_drafts + 1) * a.splits);
-  // Four elements a load where every row starts on its boundary, else one.
+  // Noise and probabilities come four a load where they lie in step with the logits: every row of all of
+  // them on its boundary.
   const uintptr_t at = (uintptr_t)a.gumbel | (a.probs ? (uintptr_t)a.probs : 0);
   const bool wide = a.ld % 4 == 0 && a.ld_gumbel % 4 == 0 && (!a.probs || a.ld_probs % 4 == 0) && !(at & 15) &&
                     !((uintptr_t)a.logits & (a.type == G4_F32 ? 15 : 7));
-  if (a.type == G4_F32) return wide ? launch_drafts<float, 4>(a, state, st) : launch_drafts<float, 1>(a, state, st);
-  return wide ? launch_drafts<__nv_bfloat16, 4>(a, state, st) : launch_drafts<__nv_bfloat16, 1>(a, state, st);
+  if (a.type == G4_F32) return wide ? launch_drafts<float, true>(a, state, st) : launch_drafts<float, false>(a, state, st);
+  return wide ? launch_drafts<__nv_bfloat16, true>(a, state, st) : launch_drafts<__nv_bfloat16, false>(a, state, st);
 }
 
 }  // namespace g4

@@ -117,9 +117,9 @@ __device__ __forceinline__ void decode8(uint2 c, float s, float (&x)[8]) {
   }
 }
 
-constexpr int kRowItems = 2;   // (token, head) pairs a thread has in flight
-
-template <typename T, int FMT, int HD>
+// kRowItems: (token, head) pairs a thread has in flight, 2 where the call fills the SMs several times over
+// (40,001 x 8 x 128 read back: 44 us against 53), else 1 (129 x 512: 2.9 us against 4.5).
+template <typename T, int FMT, int HD, int kRowItems>
 __global__ void __launch_bounds__(256)
     k_page_store(const Pool p, const T *__restrict__ k, const T *__restrict__ v, long long k_stride,
                  long long v_stride, int tokens, const int32_t *__restrict__ slots) {
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-template <typename T, int FMT, int HD>
+template <typename T, int FMT, int HD, int kRowItems>
 __global__ void __launch_bounds__(256)
     k_page_read(const Pool p, T *__restrict__ k, T *__restrict__ v, long long k_stride, long long v_stride,
                 int tokens, const int32_t *__restrict__ slots) {
@@ -260,13 +260,16 @@ template <typename T, int FMT>
 cudaError_t launch_rows(const Pool &p, bool store, void *k, void *v, long long ks, long long vs, int tokens,
                         const int32_t *slots, cudaStream_t st) {
   const int lanes = p.hd / 8 < 32 ? p.hd / 8 : 32;
-  const long long per_block = 256 / lanes * kRowItems;
-  const dim3 grid((unsigned)(((long long)tokens * p.kv_heads + per_block - 1) / per_block)), block(256);
+  const long long items = (long long)tokens * p.kv_heads, side = 256 / lanes;
+  const int n = items > side * 148 * 8 * 2 ? 2 : 1;
+  const dim3 grid((unsigned)((items + side * n - 1) / (side * n))), block(256);
   T *tk = (T *)k, *tv = (T *)v;
   auto go = [&](auto hd) {
     constexpr int HD = decltype(hd)::value;
-    return store ? launch_k(k_page_store<T, FMT, HD>, grid, block, 0, st, false, p, (const T *)tk, (const T *)tv, ks, vs, tokens, slots)
-                 : launch_k(k_page_read<T, FMT, HD>, grid, block, 0, st, false, p, tk, tv, ks, vs, tokens, slots);
+    if (store)
+      return launch_k(n == 2 ? k_page_store<T, FMT, HD, 2> : k_page_store<T, FMT, HD, 1>, grid, block, 0, st, false, p, (const T *)tk,
+                      (const T *)tv, ks, vs, tokens, slots);
+    return launch_k(n == 2 ? k_page_read<T, FMT, HD, 2> : k_page_read<T, FMT, HD, 1>, grid, block, 0, st, false, p, tk, tv, ks, vs, tokens, slots);
   };
   switch (p.hd) {
     case 64: return go(std::integral_constant<int, 64>{});

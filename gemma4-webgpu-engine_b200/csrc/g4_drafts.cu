@@ -11,6 +11,7 @@
 #include <cuda_runtime.h>
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "g4_device.cuh"
@@ -171,10 +172,11 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_scan(const DraftArgs a,
   Race best{-INFINITY, 0x7fffffff};
   const int head = before4(src);   // tokens before the first share's first load
   const int c0 = split * a.chunk + head, c1 = min(a.vocab, c0 + a.chunk);
-  constexpr int U = 4, STEP = kDraftThreads * 4;   // loads in flight of each kind
-  // One pass of 16 tokens a thread. FULL: all of them are there and none is left out.
+  constexpr int STEP = kDraftThreads * 4;
+  // One pass of 16 tokens a thread, 32 where only the logits are read: the loads in flight. FULL: all of them are there and none is left out.
   auto pass = [&](auto full_, auto race_, auto noisy_, int i0) {
     constexpr bool FULL = decltype(full_)::value, RACE = decltype(race_)::value, NOISY = decltype(noisy_)::value;
+    constexpr int U = NOISY ? 4 : 8;
     float x[U][4], g[U][4];
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -221,6 +223,7 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_scan(const DraftArgs a,
       sum = {fmaxf(x, -INFINITY), x == -INFINITY ? 0.0f : ex2(fmaf(x, kLog2e, -x * kLog2e))};
       if (decltype(race_)::value && key > best.key && t != left_out) best = {key, t};
     }
+    constexpr int U = decltype(noisy_)::value ? 4 : 8;
     for (int b0 = c0; b0 < c1; b0 += STEP * U) {
       const int i0 = b0 + t * 4;
       if (b0 + STEP * U <= c1 && (left_out < b0 || left_out >= b0 + STEP * U))
@@ -322,19 +325,24 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_rest(const DraftArgs a,
   // `s` and `m` carry the plain race here: its key, and its token as a float's bits.
   Race rest{-INFINITY, 0x7fffffff}, plain{-INFINITY, 0x7fffffff};
   const int head = before4(src), c0 = split * a.chunk + head, c1 = min(a.vocab, c0 + a.chunk);
+  float bar = -INFINITY;   // a key of this warp's: what is below it is out
   auto race = [&](int i, float x, float g, float q) {
-    const float xs = __fmul_rn(x, inv);
-    const float left = __fsub_rn(expf(__fsub_rn(xs, st.lse)), q);
-    if (left > 0.0f) {
-      const float key = __fadd_rn(logf(left), g);
-      if (key > rest.key) rest = {key, i};
-    }
-    const float key = __fadd_rn(xs, g);
+    const float xs = __fmul_rn(x, inv), lp = __fsub_rn(xs, st.lse), key = __fadd_rn(xs, g);
     if (key > plain.key) plain = {key, i};
+    // What is left is at most p, so ln left + gumbel at most ln p + gumbel (and 1e-3 covers what the
+    // functions' rounding adds): nearly every token is out of the race without either function.
+    if (__fadd_rn(lp, g) + fmaf(fabsf(xs), 1e-6f, 1e-3f) > bar) {
+      const float left = __fsub_rn(expf(lp), q);
+      if (left > 0.0f) {
+        const float k = __fadd_rn(logf(left), g);
+        if (k > rest.key) rest = {k, i};
+      }
+    }
   };
   if (split == 0 && t < head && t < a.vocab) race(t, logit_at<T>(a, st.row, t), noise[t], probs[t]);
   constexpr int U = 2, STEP = kDraftThreads * 4;
-  for (int i0 = c0 + t * 4; i0 < c1; i0 += STEP * U) {
+  for (int b0 = c0; b0 < c1; b0 += STEP * U) {
+    const int i0 = b0 + t * 4;
     float x[U][4], g[U][4], q[U][4];
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -356,7 +364,14 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_rest(const DraftArgs a,
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) race(i0 + u * STEP + e, x[u][e], g[u][e], q[u][e]);
+      for (int e = 0; e < 4; e++) {
+        race(i0 + u * STEP + e, x[u][e], g[u][e], q[u][e]);
+        if (e == 0) {
+          bar = rest.key;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) bar = fmaxf(bar, __shfl_xor_sync(0xffffffffu, bar, d));
+        }
+      }
   }
   const DraftPart r = block_join({-INFINITY, 0.0f, rest.key, rest.idx}, sh);
   __syncthreads();
@@ -393,25 +408,34 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_rest(const DraftArgs a,
   }
 }
 
-// Tokens a block scans: 16384, or fewer (in steps of 1024) until the rows fill the SMs twice.
+// Tokens a block scans: as many as let `rows` rows fill the SMs once (4 blocks each; a block costs a few
+// microseconds besides its loads: 144 rows of 262,144 took 29 us in one round, 34 and 40 in two and
+// four), at least 2048, in steps of 1024.
 static int draft_chunk(int vocab, int rows) {
-  const int want = 2 * 148 / (rows > 0 ? rows : 1);
-  int splits = (vocab + 16383) / 16384;
-  if (splits < want) splits = want;
-  const int chunk = (vocab + splits - 1) / splits;
-  return (chunk + 1023) / 1024 * 1024;
+  const int splits = std::max(1, 4 * 148 / std::max(rows, 1));
+  return std::max(2048, ((vocab + splits - 1) / splits + 1023) / 1024 * 1024);
 }
+
+// Few sequences have such a row, so its shares are small: one pass of a block.
+constexpr int kRestChunk = 2048;
 
 size_t verify_drafts_partials(int vocab, int rows, int batch, int max_drafts) {
   const int chunk = draft_chunk(vocab, rows), splits = (vocab + chunk - 1) / chunk;
-  return (size_t)batch * (max_drafts + 1) * splits * sizeof(DraftPart) + (size_t)batch * sizeof(DraftState);
+  const int rest_splits = (vocab + kRestChunk - 1) / kRestChunk;
+  const size_t scan = (size_t)(max_drafts + 1) * splits;
+  return (size_t)batch * std::max(scan, (size_t)rest_splits) * sizeof(DraftPart) + (size_t)batch * sizeof(DraftState);
 }
 
 template <typename T, bool NW>
 static cudaError_t launch_drafts(const DraftArgs &a, DraftState *state, cudaStream_t st) {
   const dim3 block(kDraftThreads);
   cudaError_t e = launch_k(k_draft_scan<T, NW>, dim3(a.splits, a.max_drafts + 1, a.batch), block, 0, st, false, a, state);
-  if (e == cudaSuccess && a.probs) e = launch_k(k_draft_rest<T, NW>, dim3(a.splits, a.batch), block, 0, st, false, a, state);
+  if (e == cudaSuccess && a.probs) {
+    DraftArgs r = a;   // one row a sequence at most: shares of its own size
+    r.chunk = kRestChunk;
+    r.splits = (a.vocab + r.chunk - 1) / r.chunk;
+    e = launch_k(k_draft_rest<T, NW>, dim3(r.splits, a.batch), block, 0, st, false, r, state);
+  }
   return e;
 }
 
@@ -419,7 +443,8 @@ cudaError_t launch_verify_drafts(const DraftArgs &args, cudaStream_t st) {
   DraftArgs a = args;
   a.chunk = draft_chunk(a.vocab, a.rows);
   a.splits = (a.vocab + a.chunk - 1) / a.chunk;
-  DraftState *state = reinterpret_cast<DraftState *>(a.part + (size_t)a.batch * (a.max_drafts + 1) * a.splits);
+  DraftState *state = reinterpret_cast<DraftState *>(
+      (char *)a.part + verify_drafts_partials(a.vocab, a.rows, a.batch, a.max_drafts) - (size_t)a.batch * sizeof(DraftState));
   // Noise and probabilities come four a load where they lie in step with the logits: every row of all of
   // them on its boundary.
   const uintptr_t at = (uintptr_t)a.gumbel | (a.probs ? (uintptr_t)a.probs : 0);

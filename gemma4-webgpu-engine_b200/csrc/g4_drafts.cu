@@ -1,7 +1,8 @@
 // g4_drafts.cu -- verification of drafted tokens against the target model's probabilities.
 //
 // With x = logits / T a draft d stands when u w < p[d] = exp(x[d] - lse), lse = m + ln sum exp(x -
-// m): one pass over the row gives m and the sum. The token that follows is a race of exponential
+// m): one pass over the row gives m and the sum. The greatest x are counted and only the others summed:
+// where one token has nearly all of p, ln p is -ln(1 + r) of a small r, and r keeps its digits. The token that follows is a race of exponential
 // clocks, argmax(ln weight + gumbel): with a certain drafter the weights of a refused row are p
 // without d, so ln weight is x itself up to a constant and the same pass over the row finds the
 // winner; no second pass and no cumulative sums, whose rounding would decide the token. Only a
@@ -42,26 +43,38 @@ struct Race {
 };
 
 struct RowSum {
-  float m, s;
-  __device__ __forceinline__ void add(float om, float os) {
-    const float n = fmaxf(m, om);
-    const float ref = n == -INFINITY ? 0.0f : n;
-    s = s * expf(m - ref) + os * expf(om - ref);
-    m = n;
+  float m, n, r;
+  __device__ __forceinline__ void add(float om, float on, float orr) {
+    if (om == m) {
+      n += on;
+      r += orr;
+      return;
+    }
+    const bool up = om > m;
+    const float hi = up ? om : m, lo = up ? m : om;
+    // (A NaN on either side stays in the sum.)
+    const float f = lo == -INFINITY ? 0.0f : ex2((lo - hi) * kLog2e);
+    r = up ? fmaf(n + r, f, orr) : fmaf(on + orr, f, r);
+    n = up ? on : n;
+    m = hi;
   }
+  // ln of the whole sum.
+  __device__ __forceinline__ float ln() const { return n == 1.0f ? log1pf(r) : logf(n + r); }
 };
+
+constexpr DraftPart kNone = {-INFINITY, 0.0f, 0.0f, -INFINITY, 0x7fffffff, {0, 0, 0}};
 
 __device__ __forceinline__ DraftPart warp_join(DraftPart v) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) {
-    const float om = __shfl_xor_sync(0xffffffffu, v.m, d), os = __shfl_xor_sync(0xffffffffu, v.s, d);
-    const float ok = __shfl_xor_sync(0xffffffffu, v.key, d);
+    const float om = __shfl_xor_sync(0xffffffffu, v.m, d), on = __shfl_xor_sync(0xffffffffu, v.n, d);
+    const float orr = __shfl_xor_sync(0xffffffffu, v.r, d), ok = __shfl_xor_sync(0xffffffffu, v.key, d);
     const int oi = __shfl_xor_sync(0xffffffffu, v.idx, d);
-    RowSum r{v.m, v.s};
-    r.add(om, os);
+    RowSum r{v.m, v.n, v.r};
+    r.add(om, on, orr);
     Race c{v.key, v.idx};
     c.add(ok, oi);
-    v = {r.m, r.s, c.key, c.idx};
+    v = {r.m, r.n, r.r, c.key, c.idx, {0, 0, 0}};
   }
   return v;
 }
@@ -71,7 +84,7 @@ __device__ __forceinline__ DraftPart block_join(DraftPart v, DraftPart *sh) {
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
   __syncthreads();
   if (threadIdx.x < 32) {
-    v = threadIdx.x < kDraftThreads / 32 ? sh[threadIdx.x] : DraftPart{-INFINITY, 0.0f, -INFINITY, 0x7fffffff};
+    v = threadIdx.x < kDraftThreads / 32 ? sh[threadIdx.x] : kNone;
     v = warp_join(v);
   }
   return v;
@@ -127,11 +140,11 @@ __device__ __forceinline__ SeqRows seq_rows(const DraftArgs &a, int b, bool repo
   return s;
 }
 
-// What the scan leaves for the remainder's race: the row that emits (-1: done), its place and lse.
+// What the scan leaves for the remainder's race: the row that emits (-1: done), its place, its greatest x
+// and ln sum exp(x - m).
 struct DraftState {
   int row, at;
-  float lse;
-  int pad;
+  float m, ln;
 };
 
 // Block (split, j, b): split's share of sequence b's row j. The sequence's last block to finish
@@ -168,7 +181,7 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_scan(const DraftArgs a,
   const bool race = greedy || final_row || !a.probs, noisy = race && !greedy;
   const T *src = reinterpret_cast<const T *>(a.logits) + row * a.ld;
   const float *noise = a.gumbel + (long long)b * a.ld_gumbel;
-  RowSum sum{-INFINITY, 0.0f};
+  RowSum sum{-INFINITY, 0.0f, 0.0f};
   Race best{-INFINITY, 0x7fffffff};
   const int head = before4(src);   // tokens before the first share's first load
   const int c0 = split * a.chunk + head, c1 = min(a.vocab, c0 + a.chunk);
@@ -200,27 +213,35 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_scan(const DraftArgs a,
         x[u][e] = __fmul_rn(x[u][e], inv);
         top = fmaxf(top, x[u][e]);
       }
-    const float ref = top == -INFINITY ? 0.0f : top, low = -ref * kLog2e;
-    float s0 = sum.s * ex2(fmaf(sum.m, kLog2e, low)), s1 = 0.0f;
+    // (A row of nothing but -inf so far: ref 0, and every term is 0.)
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float n = sum.n, s0 = sum.r, s1 = 0.0f;
+    if (top != sum.m) {
+      s0 = sum.m == -INFINITY ? s0 : (n + s0) * ex2((sum.m - ref) * kLog2e);
+      n = 0.0f;
+    }
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        (e & 1 ? s1 : s0) += ex2(fmaf(x[u][e], kLog2e, low));
+        const float p = ex2((x[u][e] - ref) * kLog2e);
+        const bool is_top = x[u][e] == top;
+        n += is_top ? 1.0f : 0.0f;
+        (e & 1 ? s1 : s0) += is_top ? 0.0f : p;
         if (RACE) {
           const int i = i0 + u * STEP + e;
           const float key = NOISY ? __fadd_rn(x[u][e], g[u][e]) : x[u][e];
           if (key > best.key && (FULL || i != left_out)) best = {key, i};
         }
       }
-    sum = {top, s0 + s1};
+    sum = {top, n, s0 + s1};
   };
   auto passes = [&](auto race_, auto noisy_) {
     if (split == 0 && t < head && t < a.vocab) {
       const float x = __fmul_rn(logit_at<T>(a, row, t), inv);
       const float key = decltype(noisy_)::value ? __fadd_rn(x, noise[t]) : x;
       // (A NaN makes the row's sum one, as in the passes.)
-      sum = {fmaxf(x, -INFINITY), x == -INFINITY ? 0.0f : ex2(fmaf(x, kLog2e, -x * kLog2e))};
+      sum = x != x ? RowSum{-INFINITY, 0.0f, x} : RowSum{x, 1.0f, 0.0f};
       if (decltype(race_)::value && key > best.key && t != left_out) best = {key, t};
     }
     constexpr int U = decltype(noisy_)::value ? 4 : 8;
@@ -238,7 +259,7 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_scan(const DraftArgs a,
     passes(std::true_type{}, std::false_type{});
   else
     passes(std::false_type{}, std::false_type{});
-  DraftPart v = block_join({sum.m, sum.s, best.key, best.idx}, sh);
+  DraftPart v = block_join({sum.m, sum.n, sum.r, best.key, best.idx, {0, 0, 0}}, sh);
   DraftPart *parts = a.part + ((long long)b * width + j) * a.splits;
   if (t == 0) {
     parts[split] = v;
@@ -250,24 +271,24 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_scan(const DraftArgs a,
   __threadfence();
 
   // Every row's sums, one warp a row; then the first draft that does not stand.
-  __shared__ float lse[kMaxDrafts + 1], lp[kMaxDrafts + 1];
+  __shared__ float row_m[kMaxDrafts + 1], row_ln[kMaxDrafts + 1], lp[kMaxDrafts + 1];
   __shared__ int chosen[kMaxDrafts + 1];
   __shared__ bool stands[kMaxDrafts + 1];
   const int warp = t >> 5, lane = t & 31;
   for (int r = warp; r < sr.n; r += kDraftThreads / 32) {
     const DraftPart *rp = a.part + ((long long)b * width + r) * a.splits;
-    DraftPart w{-INFINITY, 0.0f, -INFINITY, 0x7fffffff};
+    DraftPart w = kNone;
     for (int s = lane; s < a.splits; s += 32) {
       const float4 f = __ldcg(reinterpret_cast<const float4 *>(rp + s));
-      RowSum rs{w.m, w.s};
-      rs.add(f.x, f.y);
+      RowSum rs{w.m, w.n, w.r};
+      rs.add(f.x, f.y, f.z);
       Race c{w.key, w.idx};
-      c.add(f.z, __float_as_int(f.w));
-      w = {rs.m, rs.s, c.key, c.idx};
+      c.add(f.w, __ldcg(&rp[s].idx));
+      w = {rs.m, rs.n, rs.r, c.key, c.idx, {0, 0, 0}};
     }
     w = warp_join(w);
     if (lane == 0) {
-      const float ln = logf(w.s);
+      const float ln = RowSum{w.m, w.n, w.r}.ln();
       const int pick = w.idx == 0x7fffffff ? 0 : w.idx;
       bool ok = false;
       float lpd = 0.0f;
@@ -286,7 +307,8 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_scan(const DraftArgs a,
       stands[r] = ok;
       chosen[r] = pick;
       lp[r] = lpd;
-      lse[r] = w.m + ln;
+      row_m[r] = w.m;
+      row_ln[r] = ln;
       // ln p of the row's winner, for the row that emits it.
       if (!ok) lp[r] = (__fmul_rn(logit_at<T>(a, sr.row + r, pick), inv) - w.m) - ln;
     }
@@ -300,7 +322,7 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_scan(const DraftArgs a,
     a.count[b] = 0;
     a.counts[b] = r + 1;
     const bool rest = a.probs && !greedy && r < sr.n - 1;
-    state[b] = {rest ? sr.row + r : -1, r, lse[r], 0};
+    state[b] = {rest ? sr.row + r : -1, r, row_m[r], row_ln[r]};
   }
   __syncthreads();
   for (int i = t; i < width; i += kDraftThreads) {
@@ -322,12 +344,11 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_rest(const DraftArgs a,
   const T *src = reinterpret_cast<const T *>(a.logits) + (long long)st.row * a.ld;
   const float *noise = a.gumbel + (long long)b * a.ld_gumbel;
   const float *probs = a.probs + (long long)st.row * a.ld_probs;
-  // `s` and `m` carry the plain race here: its key, and its token as a float's bits.
   Race rest{-INFINITY, 0x7fffffff}, plain{-INFINITY, 0x7fffffff};
   const int head = before4(src), c0 = split * a.chunk + head, c1 = min(a.vocab, c0 + a.chunk);
   float bar = -INFINITY;   // a key of this warp's: what is below it is out
   auto race = [&](int i, float x, float g, float q) {
-    const float xs = __fmul_rn(x, inv), lp = __fsub_rn(xs, st.lse), key = __fadd_rn(xs, g);
+    const float xs = __fmul_rn(x, inv), lp = __fsub_rn(__fsub_rn(xs, st.m), st.ln), key = __fadd_rn(xs, g);
     if (key > plain.key) plain = {key, i};
     // What is left is at most p, so ln left + gumbel at most ln p + gumbel (and 1e-3 covers what the
     // functions' rounding adds): nearly every token is out of the race without either function.
@@ -373,12 +394,12 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_rest(const DraftArgs a,
         }
       }
   }
-  const DraftPart r = block_join({-INFINITY, 0.0f, rest.key, rest.idx}, sh);
+  const DraftPart r = block_join({-INFINITY, 0.0f, 0.0f, rest.key, rest.idx, {0, 0, 0}}, sh);
   __syncthreads();
-  const DraftPart p = block_join({-INFINITY, 0.0f, plain.key, plain.idx}, sh);
+  const DraftPart p = block_join({-INFINITY, 0.0f, 0.0f, plain.key, plain.idx, {0, 0, 0}}, sh);
   DraftPart *parts = a.part + (long long)b * a.splits;
   if (t == 0) {
-    parts[split] = {p.key, __int_as_float(p.idx), r.key, r.idx};
+    parts[split] = {p.key, __int_as_float(p.idx), r.key, __int_as_float(r.idx), 0, {0, 0, 0}};
     __threadfence();
     last_block = atomicAdd(a.count + b, 1u) == (unsigned)a.splits - 1;
   }
@@ -404,7 +425,7 @@ __global__ void __launch_bounds__(kDraftThreads) k_draft_rest(const DraftArgs a,
     const long long at = (long long)b * (a.max_drafts + 1) + st.at;
     a.count[b] = 0;
     a.tokens[at] = pick;
-    a.logprobs[at] = __fsub_rn(__fmul_rn(logit_at<T>(a, st.row, pick), inv), st.lse);
+    a.logprobs[at] = __fsub_rn(__fsub_rn(__fmul_rn(logit_at<T>(a, st.row, pick), inv), st.m), st.ln);
   }
 }
 

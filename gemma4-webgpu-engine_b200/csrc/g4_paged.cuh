@@ -57,10 +57,11 @@ struct DraftArgs {
   uint32_t *count;
   int *err;
 };
-// One block's share of a row: the greatest x, the sum of exp(x - m), the winner of the race.
+// One block's share of a row: the greatest x, how many are equal to it, the sum of exp(x - m) over the
+// others, the winner of the race.
 struct __align__(16) DraftPart {
-  float m, s, key;
-  int idx;
+  float m, n, r, key;
+  int idx, pad[3];
 };
 
 // Every workspace starts with this many zeroed counters; a kernel that counts its finished blocks

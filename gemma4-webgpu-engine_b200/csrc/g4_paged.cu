@@ -79,7 +79,10 @@ struct Eight<__nv_bfloat16> {
   }
 };
 
-// Codes of eight values (scale s, 0 or NaN: codes 0).
+// Codes of eight values (scale s, 0 or NaN: codes 0): that of the correctly rounded quotient x / s. The
+// divisions bind the kernel by instructions (82% of issue slots); multiplying by the reciprocal and
+// dividing only next to the middle between two codes lost, as bf16 rows lie there often (16,389 x 8 x 128
+// stored and read back: e4m3 57 us against 51).
 template <int FMT>
 __device__ __forceinline__ uint2 encode8(const float (&x)[8], float s) {
   uint32_t w[2] = {0, 0};
@@ -167,22 +170,18 @@ __global__ void __launch_bounds__(256)
         }
         continue;
       }
-      // The greatest magnitude over the row; x - x is 0 unless x is an infinity or a NaN.
-      float top = 0.0f;
-      bool bad = false;
+      // The greatest magnitude over the row: magnitudes order as their bits do, infinities and NaN last.
+      uint32_t most = 0;
 #pragma unroll
       for (int c = 0; c < CH; c++) {
         float x[8];
         in[n][w][c].get(x);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          top = fmaxf(top, fabsf(x[i]));
-          bad |= !(__fsub_rn(x[i], x[i]) == 0.0f);
-        }
+        for (int i = 0; i < 8; i++) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
       }
-      if (bad) top = __int_as_float(0x7f800000);
 #pragma unroll
-      for (int m = 1; m < LR; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+      for (int m = 1; m < LR; m <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, m));
+      const float top = __uint_as_float(min(most, 0x7f800000u));
       float s = __fdiv_rn(top, FMT == G4_PAGE_INT8 ? 127.0f : 448.0f);
       if (s == __int_as_float(0x7f800000)) s = __int_as_float(0x7fffffff);
       if (on) {

@@ -38,10 +38,10 @@
 namespace g4 {
 
 constexpr int kDecWarps = 4;
-#ifndef SPLIT_T
-#define SPLIT_T 3
-#define BEGIN_T 16
-#endif
+// The list's units (plan_decode): what beginning a context costs, in tiles (64 x 4,096 at head_dim 256 47 us
+// at 6, 45 at 12; 64 ragged at head_dim 512 67 at 1, 53 at 12 and 52 at 16), and the least share of a
+// block, in tiles a warp (1 x 2,000: 18 us at 3, 19 at 5, 24 at 8).
+constexpr int kBeginTiles = 16, kLeastTiles = 3;
 constexpr int kRingKb = 96;          // of an SM's shared memory in rings
 constexpr int kJoin = 16;            // partials one block joins
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
@@ -323,516 +323,516 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
 
 #pragma unroll 1
   while (at < end) {
-  // ---- the part at hand: KV head and row group of sequence b, its tiles tile0 .. tile1 - 1.
-  const SeqSpan s = seq_span(a, b, false);
-  int kvh = 0, rg = 0, first = 0, tiles;
-  long long item_at = seq_at;
-  {
-    int all = 0;
-    for (int r = 0; r < a.row_groups; r++) all += tiles_of(s, r, first);
-    if (at >= seq_at + (long long)all * p.kv_heads) {   // this sequence is done
-      seq_at += (long long)all * p.kv_heads;
-      b++;
+    // ---- the part at hand: KV head and row group of sequence b, its tiles tile0 .. tile1 - 1.
+    const SeqSpan s = seq_span(a, b, false);
+    int kvh = 0, rg = 0, first = 0, tiles;
+    long long item_at = seq_at;
+    {
+      int all = 0;
+      for (int r = 0; r < a.row_groups; r++) all += tiles_of(s, r, first);
+      if (at >= seq_at + (long long)all * p.kv_heads) {   // this sequence is done
+        seq_at += (long long)all * p.kv_heads;
+        b++;
+        continue;
+      }
+      kvh = (int)((at - seq_at) / all);
+      item_at += (long long)kvh * all;
+      tiles = tiles_of(s, 0, first);
+      while (at >= item_at + tiles) {
+        item_at += tiles;
+        tiles = tiles_of(s, ++rg, first);
+      }
+    }
+    const int R = s.n * a.group, row0 = rg * ROWS;
+    const int from = (int)(at - item_at), count = (int)min((long long)tiles - from, end - at);
+    // The share may end among the tiles that stand for the beginning: then there is nothing to do here.
+    const int begin = a.begin_tiles, real = tiles - begin;
+    const int tile0 = first + max(from - begin, 0), tile1 = first + max(from + count - begin, 0);
+    if (real > 0 && tile1 == tile0) {
+      at += count;
       continue;
     }
-    kvh = (int)((at - seq_at) / all);
-    item_at += (long long)kvh * all;
-    tiles = tiles_of(s, 0, first);
-    while (at >= item_at + tiles) {
-      item_at += tiles;
-      tiles = tiles_of(s, ++rg, first);
-    }
-  }
-  const int R = s.n * a.group, row0 = rg * ROWS;
-  const int from = (int)(at - item_at), count = (int)min((long long)tiles - from, end - at);
-  // The share may end among the tiles that stand for the beginning: then there is nothing to do here.
-  const int begin = a.begin_tiles, real = tiles - begin;
-  const int tile0 = first + max(from - begin, 0), tile1 = first + max(from + count - begin, 0);
-  if (real > 0 && tile1 == tile0) {
-    at += count;
-    continue;
-  }
-  const bool complete = tile1 - tile0 == real;
+    const bool complete = tile1 - tile0 == real;
 
-  // ---- this group's tiles: tile0 + tg + TG n; its first warp asks for them.
-  const int mine = tile1 - tile0 - tg > 0 ? (tile1 - tile0 - tg + TG - 1) / TG : 0;
-  const int32_t *table = a.table + (long long)b * a.table_stride;
-  // Lane i of the first warp holds where the rows of the i-th of 32 tiles from pages_at on lie in the
-  // pool (-1: no such page), so that asking for one is a shuffle and the copies.
-  long long rows = -1;
-  int pages_at = 0;
-  auto fetch_pages = [&](int n) {
-    const int k = n + lane;
-    rows = -1;
-    if (k < mine) {
-      const int tile = tile0 + tg + TG * k, of = tile / per_page;
-      const int page = table[of];
-      if (page < 0 || page >= p.n_pages)
-        paged_raise(a.err, G4_PAGED_BAD_PAGE);
-      else
-        rows = ((long long)page * p.kv_heads + kvh) * p.page_size + (tile - of * per_page) * 16;
-    }
-    pages_at = n;
-  };
-  if (rt == 0 && mine > 0) fetch_pages(0);
-
-  // ---- Q: its loads go out before the first positions are asked for. One warp a row, two rows at a
-  // time; a lane takes four dimensions of each 128.
-  constexpr int QC = (HD + 127) / 128;
-  float4 qv[2][QC];
-  auto load_q = [&](int r, float4 (&v)[QC]) {
-    const int rr = row0 + r, i = rr / a.group;
-#pragma unroll
-    for (int j = 0; j < QC; j++) {
-      const int d = 128 * j + 4 * lane;
-      v[j] = make_float4(0, 0, 0, 0);
-      if (rr < R && d < HD) {
-        const long long from = (long long)(s.row + i) * a.q_stride + (long long)(kvh * a.group + rr % a.group) * HD + d;
-        if (a.type == G4_F32) {
-          v[j] = *reinterpret_cast<const float4 *>((const float *)a.q + from);
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2 *>((const __nv_bfloat16 *)a.q + from);
-          v[j] = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                             __uint_as_float(u.y & 0xffff0000u));
-        }
+    // ---- this group's tiles: tile0 + tg + TG n; its first warp asks for them.
+    const int mine = tile1 - tile0 - tg > 0 ? (tile1 - tile0 - tg + TG - 1) / TG : 0;
+    const int32_t *table = a.table + (long long)b * a.table_stride;
+    // Lane i of the first warp holds where the rows of the i-th of 32 tiles from pages_at on lie in the
+    // pool (-1: no such page), so that asking for one is a shuffle and the copies.
+    long long rows = -1;
+    int pages_at = 0;
+    auto fetch_pages = [&](int n) {
+      const int k = n + lane;
+      rows = -1;
+      if (k < mine) {
+        const int tile = tile0 + tg + TG * k, of = tile / per_page;
+        const int page = table[of];
+        if (page < 0 || page >= p.n_pages)
+          paged_raise(a.err, G4_PAGED_BAD_PAGE);
+        else
+          rows = ((long long)page * p.kv_heads + kvh) * p.page_size + (tile - of * per_page) * 16;
       }
-    }
-  };
-  load_q(warp, qv[0]);
-  load_q(warp + kDecWarps, qv[1]);
+      pages_at = n;
+    };
+    if (rt == 0 && mine > 0) fetch_pages(0);
 
-  // Unit u of the group (K of tile u / 2, or V) into slot sl, by its whole first warp.
-  auto request = [&](int u, int sl) {
-    const int n = u >> 1;
-    if (n >= mine) return;
-    if (n - pages_at >= 32) fetch_pages(n);
-    const long long row = __shfl_sync(0xffffffffu, rows, n - pages_at);
-    if (lane != 0) return;
-    has[sl] = row >= 0;
-    if (row < 0) {
-      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&full[sl])) : "memory");
-      return;
-    }
-    uint8_t *to = ring + sl * S::UNIT;
-    const bool is_v = u & 1;
-    mbar_expect_tx(&full[sl], 16 * S::ROW + (HALF && !is_v ? 128 : 0));
-    bulk_g2s(to, (is_v ? p.v : p.k) + row * S::ROW, 16 * S::ROW, &full[sl]);
-    if (HALF && !is_v) {
-      bulk_g2s(to + 16 * S::ROW, p.ks + row, 64, &full[sl]);
-      bulk_g2s(to + 16 * S::ROW + 64, p.vs + row, 64, &full[sl]);
-    }
-  };
-  const int sl0 = ubase % D;   // the first unit's slot
-  if (rt == 0)
-    for (int u = 0; u < D; u++) request(u, sl0 + u < D ? sl0 + u : sl0 + u - D);
-
-  // Q into fragment order: for K step k of row tile r lane (g, c) holds four consecutive dimensions of
-  // row g. 8-bit pages: f16 parts, scaled by a power of two that takes the row's greatest to 2^8 .. 2^9.
-#pragma unroll 1
-  for (int r0 = warp; r0 < ROWS; r0 += 2 * kDecWarps) {
-    if (r0 > warp) {
-      load_q(r0, qv[0]);
-      load_q(r0 + kDecWarps, qv[1]);
-    }
-#pragma unroll
-    for (int z = 0; z < 2; z++) {
-      const int r = r0 + z * kDecWarps;
-      float top = 0.0f;
-#pragma unroll
-      for (int j = 0; j < QC; j++)
-        top = fmaxf(fmaxf(fmaxf(top, fabsf(qv[z][j].x)), fmaxf(fabsf(qv[z][j].y), fabsf(qv[z][j].z))), fabsf(qv[z][j].w));
-      int e = 0;
-      if (HALF) {
-        // (Magnitudes order as their bits do.) Infinities and NaN stay what they are at any scale.
-        e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23) - 127;
-        e = e < -110 ? -110 : (e > 127 ? 0 : e);
-      }
-      const float f = HALF ? __uint_as_float((uint32_t)(127 + 8 - e) << 23) : 1.0f;
+    // ---- Q: its loads go out before the first positions are asked for. One warp a row, two rows at a
+    // time; a lane takes four dimensions of each 128.
+    constexpr int QC = (HD + 127) / 128;
+    float4 qv[2][QC];
+    auto load_q = [&](int r, float4 (&v)[QC]) {
+      const int rr = row0 + r, i = rr / a.group;
 #pragma unroll
       for (int j = 0; j < QC; j++) {
         const int d = 128 * j + 4 * lane;
-        uint32_t p01[NP], p23[NP];
-        split2<HALF, NP>(qv[z][j].x * f, qv[z][j].y * f, p01);
-        split2<HALF, NP>(qv[z][j].z * f, qv[z][j].w * f, p23);
-        // 8 bit: d = 64 m + 16 c + 4 j, step 4 m + j; 16 bit: d = 32 m + 8 c + 4 j, step 2 m + j.
-        const int step = HALF ? (d >> 6) * 4 + ((d >> 2) & 3) : (d >> 5) * 2 + ((d >> 2) & 1);
-        const int cc = HALF ? (d >> 4) & 3 : (d >> 3) & 3;
-        if (d < HD && r < ROWS) {
-#pragma unroll
-          for (int k = 0; k < NP; k++)
-            qs[(((r >> 3) * NP + k) * S::KSTEPS + step) * 32 + (r & 7) * 4 + cc] = make_uint2(p01[k], p23[k]);
+        v[j] = make_float4(0, 0, 0, 0);
+        if (rr < R && d < HD) {
+          const long long from = (long long)(s.row + i) * a.q_stride + (long long)(kvh * a.group + rr % a.group) * HD + d;
+          if (a.type == G4_F32) {
+            v[j] = *reinterpret_cast<const float4 *>((const float *)a.q + from);
+          } else {
+            const uint2 u = *reinterpret_cast<const uint2 *>((const __nv_bfloat16 *)a.q + from);
+            v[j] = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                               __uint_as_float(u.y & 0xffff0000u));
+          }
         }
       }
-      if (lane == 0 && r < ROWS) {
-        q_scale[r] = a.scale * kLog2e * (HALF ? __uint_as_float((uint32_t)(127 - 8 + e) << 23) : 1.0f);
-        int x0 = 0, x1 = 0;
-        if (row0 + r < R) row_range(a, s.pos + (row0 + r) / a.group, s.kv, x0, x1);
-        row_lo[r] = x0;
-        row_hi[r] = x1;
+    };
+    load_q(warp, qv[0]);
+    load_q(warp + kDecWarps, qv[1]);
+
+    // Unit u of the group (K of tile u / 2, or V) into slot sl, by its whole first warp.
+    auto request = [&](int u, int sl) {
+      const int n = u >> 1;
+      if (n >= mine) return;
+      if (n - pages_at >= 32) fetch_pages(n);
+      const long long row = __shfl_sync(0xffffffffu, rows, n - pages_at);
+      if (lane != 0) return;
+      has[sl] = row >= 0;
+      if (row < 0) {
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&full[sl])) : "memory");
+        return;
+      }
+      uint8_t *to = ring + sl * S::UNIT;
+      const bool is_v = u & 1;
+      mbar_expect_tx(&full[sl], 16 * S::ROW + (HALF && !is_v ? 128 : 0));
+      bulk_g2s(to, (is_v ? p.v : p.k) + row * S::ROW, 16 * S::ROW, &full[sl]);
+      if (HALF && !is_v) {
+        bulk_g2s(to + 16 * S::ROW, p.ks + row, 64, &full[sl]);
+        bulk_g2s(to + 16 * S::ROW + 64, p.vs + row, 64, &full[sl]);
+      }
+    };
+    const int sl0 = ubase % D;   // the first unit's slot
+    if (rt == 0)
+      for (int u = 0; u < D; u++) request(u, sl0 + u < D ? sl0 + u : sl0 + u - D);
+
+    // Q into fragment order: for K step k of row tile r lane (g, c) holds four consecutive dimensions of
+    // row g. 8-bit pages: f16 parts, scaled by a power of two that takes the row's greatest to 2^8 .. 2^9.
+#pragma unroll 1
+    for (int r0 = warp; r0 < ROWS; r0 += 2 * kDecWarps) {
+      if (r0 > warp) {
+        load_q(r0, qv[0]);
+        load_q(r0 + kDecWarps, qv[1]);
+      }
+#pragma unroll
+      for (int z = 0; z < 2; z++) {
+        const int r = r0 + z * kDecWarps;
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < QC; j++)
+          top = fmaxf(fmaxf(fmaxf(top, fabsf(qv[z][j].x)), fmaxf(fabsf(qv[z][j].y), fabsf(qv[z][j].z))), fabsf(qv[z][j].w));
+        int e = 0;
+        if (HALF) {
+          // (Magnitudes order as their bits do.) Infinities and NaN stay what they are at any scale.
+          e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23) - 127;
+          e = e < -110 ? -110 : (e > 127 ? 0 : e);
+        }
+        const float f = HALF ? __uint_as_float((uint32_t)(127 + 8 - e) << 23) : 1.0f;
+#pragma unroll
+        for (int j = 0; j < QC; j++) {
+          const int d = 128 * j + 4 * lane;
+          uint32_t p01[NP], p23[NP];
+          split2<HALF, NP>(qv[z][j].x * f, qv[z][j].y * f, p01);
+          split2<HALF, NP>(qv[z][j].z * f, qv[z][j].w * f, p23);
+          // 8 bit: d = 64 m + 16 c + 4 j, step 4 m + j; 16 bit: d = 32 m + 8 c + 4 j, step 2 m + j.
+          const int step = HALF ? (d >> 6) * 4 + ((d >> 2) & 3) : (d >> 5) * 2 + ((d >> 2) & 1);
+          const int cc = HALF ? (d >> 4) & 3 : (d >> 3) & 3;
+          if (d < HD && r < ROWS) {
+#pragma unroll
+            for (int k = 0; k < NP; k++)
+              qs[(((r >> 3) * NP + k) * S::KSTEPS + step) * 32 + (r & 7) * 4 + cc] = make_uint2(p01[k], p23[k]);
+          }
+        }
+        if (lane == 0 && r < ROWS) {
+          q_scale[r] = a.scale * kLog2e * (HALF ? __uint_as_float((uint32_t)(127 - 8 + e) << 23) : 1.0f);
+          int x0 = 0, x1 = 0;
+          if (row0 + r < R) row_range(a, s.pos + (row0 + r) / a.group, s.kv, x0, x1);
+          row_lo[r] = x0;
+          row_hi[r] = x1;
+        }
       }
     }
-  }
-  __syncthreads();
+    __syncthreads();
 
-  const float qf0 = q_scale[rt * 8 + 2 * c], qf1 = q_scale[rt * 8 + 2 * c + 1];
-  const int lo0 = row_lo[rt * 8 + 2 * c], hi0 = row_hi[rt * 8 + 2 * c];
-  const int lo1 = row_lo[rt * 8 + 2 * c + 1], hi1 = row_hi[rt * 8 + 2 * c + 1];
-  // Positions that every row of this warp sees need no mask.
-  const int rv = min(8, R - row0 - rt * 8);   // rows of this warp's tile that exist
-  int all_lo = 0, all_hi = 0;
-  if (rv > 0) {
-    all_lo = row_lo[rt * 8 + rv - 1];
-    all_hi = row_hi[rt * 8];
-  }
+    const float qf0 = q_scale[rt * 8 + 2 * c], qf1 = q_scale[rt * 8 + 2 * c + 1];
+    const int lo0 = row_lo[rt * 8 + 2 * c], hi0 = row_hi[rt * 8 + 2 * c];
+    const int lo1 = row_lo[rt * 8 + 2 * c + 1], hi1 = row_hi[rt * 8 + 2 * c + 1];
+    // Positions that every row of this warp sees need no mask.
+    const int rv = min(8, R - row0 - rt * 8);   // rows of this warp's tile that exist
+    int all_lo = 0, all_hi = 0;
+    if (rv > 0) {
+      all_lo = row_lo[rt * 8 + rv - 1];
+      all_hi = row_hi[rt * 8];
+    }
 
-  float o[HD / 16][4];
+    float o[HD / 16][4];
 #pragma unroll
-  for (int i = 0; i < HD / 16; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+    for (int i = 0; i < HD / 16; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
 
-  // This warp is done with unit u in slot sl; the first warp of the group asks for the unit that takes its
-  // place.
-  auto release = [&](int u, int sl, uint32_t round) {
-    __syncwarp();
-    if (RT > 1) {
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&empty[sl])) : "memory");
-      if (rt == 0 && (u + D) >> 1 < mine) wait(&empty[sl], round);
+    // This warp is done with unit u in slot sl; the first warp of the group asks for the unit that takes its
+    // place.
+    auto release = [&](int u, int sl, uint32_t round) {
       __syncwarp();
-    }
-    if (rt == 0) request(u + D, sl);
-  };
-  int sl = sl0;                                       // the ring's slot at hand and its round
-  uint32_t round = (uint32_t)(ubase / D) & 1;
-  auto advance = [&] {
-    if (++sl == D) {
-      sl = 0;
-      round ^= 1;
-    }
-  };
+      if (RT > 1) {
+        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&empty[sl])) : "memory");
+        if (rt == 0 && (u + D) >> 1 < mine) wait(&empty[sl], round);
+        __syncwarp();
+      }
+      if (rt == 0) request(u + D, sl);
+    };
+    int sl = sl0;                                       // the ring's slot at hand and its round
+    uint32_t round = (uint32_t)(ubase / D) & 1;
+    auto advance = [&] {
+      if (++sl == D) {
+        sl = 0;
+        round ^= 1;
+      }
+    };
 
 #pragma unroll 1
-  for (int n = 0; n < mine; n++) {
-    const int pos0 = (tile0 + tg + TG * n) * 16;
-    wait(&full[sl], round);
-    const bool on = has[sl];
-    float sc[4][4] = {};
-    float ks0 = 1.0f, ks1 = 1.0f, w0 = 1.0f, w1 = 1.0f;
-    const uint8_t *unit = ring + sl * S::UNIT;
-    if (on) {
-      const uint8_t *kp = unit + g * S::ROW + c * 16;
-      if (HALF) {
-        const float *f = reinterpret_cast<const float *>(unit + 16 * S::ROW);
-        ks0 = f[g];
-        ks1 = f[g + 8];
-        w0 = f[16 + g];
-        w1 = f[24 + g];
-      }
-      constexpr int ST = HALF ? 4 : 2;
+    for (int n = 0; n < mine; n++) {
+      const int pos0 = (tile0 + tg + TG * n) * 16;
+      wait(&full[sl], round);
+      const bool on = has[sl];
+      float sc[4][4] = {};
+      float ks0 = 1.0f, ks1 = 1.0f, w0 = 1.0f, w1 = 1.0f;
+      const uint8_t *unit = ring + sl * S::UNIT;
+      if (on) {
+        const uint8_t *kp = unit + g * S::ROW + c * 16;
+        if (HALF) {
+          const float *f = reinterpret_cast<const float *>(unit + 16 * S::ROW);
+          ks0 = f[g];
+          ks1 = f[g + 8];
+          w0 = f[16 + g];
+          w1 = f[24 + g];
+        }
+        constexpr int ST = HALF ? 4 : 2;
 #pragma unroll 2
-      for (int m = 0; m < S::ROW / 64; m++) {
-        const uint4 x = lds16(kp + 64 * m), y = lds16(kp + 64 * m + 8 * S::ROW);
-        const uint32_t r0[4] = {x.x, x.y, x.z, x.w}, r1[4] = {y.x, y.y, y.z, y.w};
+        for (int m = 0; m < S::ROW / 64; m++) {
+          const uint4 x = lds16(kp + 64 * m), y = lds16(kp + 64 * m + 8 * S::ROW);
+          const uint32_t r0[4] = {x.x, x.y, x.z, x.w}, r1[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-        for (int j = 0; j < ST; j++) {
-          uint32_t a0, a1, a2, a3;
-          if constexpr (HALF) {
-            codes4<FMT>(r0[j], a0, a2);
-            codes4<FMT>(r1[j], a1, a3);
-          } else {
-            a0 = r0[2 * j];
-            a2 = r0[2 * j + 1];
-            a1 = r1[2 * j];
-            a3 = r1[2 * j + 1];
-          }
+          for (int j = 0; j < ST; j++) {
+            uint32_t a0, a1, a2, a3;
+            if constexpr (HALF) {
+              codes4<FMT>(r0[j], a0, a2);
+              codes4<FMT>(r1[j], a1, a3);
+            } else {
+              a0 = r0[2 * j];
+              a2 = r0[2 * j + 1];
+              a1 = r1[2 * j];
+              a3 = r1[2 * j + 1];
+            }
 #pragma unroll
-          for (int k = 0; k < NP; k++) {
-            const uint2 bq = qw[(k * S::KSTEPS + m * ST + j) * 32];
-            mma16816<HALF>(sc[(m * ST + j) & 3], a0, a1, a2, a3, bq.x, bq.y);
-          }
-        }
-      }
-    }
-    release(2 * n, sl, round);
-    advance();
-    // ---- softmax of the tile: sums 0, 1 are position g of rows 2c, 2c + 1; 2, 3 position g + 8.
-    float sa[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) sa[i] = (sc[0][i] + sc[1][i]) + (sc[2][i] + sc[3][i]);
-    float s0 = sa[0] * (ks0 * qf0), s1 = sa[1] * (ks0 * qf1), s2 = sa[2] * (ks1 * qf0), s3 = sa[3] * (ks1 * qf1);
-    bool see0 = on, see1 = on, see2 = on, see3 = on;
-    const bool whole = on && pos0 >= all_lo && pos0 + 16 <= all_hi;
-    uint32_t dead = 0;   // positions that no row of the warp sees
-    if (!whole && on) {
-      const int t0 = pos0 + g, t1 = t0 + 8;
-      see0 = t0 >= lo0 && t0 < hi0;
-      see1 = t0 >= lo1 && t0 < hi1;
-      see2 = t1 >= lo0 && t1 < hi0;
-      see3 = t1 >= lo1 && t1 < hi1;
-      const unsigned live0 = __ballot_sync(0xffffffffu, see0 || see1), live1 = __ballot_sync(0xffffffffu, see2 || see3);
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        if (!((live0 >> (4 * i)) & 0xf)) dead |= 1u << i;
-        if (!((live1 >> (4 * i)) & 0xf)) dead |= 1u << (i + 8);
-      }
-    }
-    const float g0 = HALF ? __log2f(fmaxf(w0, 0x1p-100f)) : 0.0f, g1 = HALF ? __log2f(fmaxf(w1, 0x1p-100f)) : 0.0f;
-    s0 = see0 ? s0 : -INFINITY;
-    s1 = see1 ? s1 : -INFINITY;
-    s2 = see2 ? s2 : -INFINITY;
-    s3 = see3 ? s3 : -INFINITY;
-    float n0 = fmaxf(s0 + g0, s2 + g1), n1 = fmaxf(s1 + g0, s3 + g1);
-#pragma unroll
-    for (int x = 4; x < 32; x <<= 1) {
-      n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
-      n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
-    }
-    n0 = fmaxf(n0, m0);
-    n1 = fmaxf(n1, m1);
-    if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
-      const float f0 = n0 > m0 ? ex2(m0 - n0) : 1.0f, f1 = n1 > m1 ? ex2(m1 - n1) : 1.0f;
-      l0 = n0 > m0 ? rescale(l0, m0 - n0) : l0;
-      l1 = n1 > m1 ? rescale(l1, m1 - n1) : l1;
-#pragma unroll
-      for (int i = 0; i < HD / 16; i++) {
-        o[i][0] *= f0;
-        o[i][1] *= f1;
-        o[i][2] *= f0;
-        o[i][3] *= f1;
-      }
-      m0 = n0;
-      m1 = n1;
-    }
-    uint32_t pw[2][NP];
-    {
-      const float bits = HALF ? kWeightBits : 0.0f;
-      const float r0 = m0 == -INFINITY ? 0.0f : m0 - bits, r1 = m1 == -INFINITY ? 0.0f : m1 - bits;
-      const float p0 = ex2(s0 - r0), p1 = ex2(s1 - r1), p2 = ex2(s2 - r0), p3 = ex2(s3 - r1);
-      l0 += p0 + p2;
-      l1 += p1 + p3;
-      uint32_t x[NP], y[NP];
-      split2<HALF, NP>(see0 ? p0 * w0 : 0.0f, see1 ? p1 * w0 : 0.0f, x);
-      split2<HALF, NP>(see2 ? p2 * w1 : 0.0f, see3 ? p3 * w1 : 0.0f, y);
-#pragma unroll
-      for (int k = 0; k < NP; k++) {
-        pw[0][k] = transpose8x8(x[k]);
-        pw[1][k] = transpose8x8(y[k]);
-      }
-    }
-    wait(&full[sl], round);
-    if (on) {
-      const uint8_t *vp = ring + sl * S::UNIT + 2 * c * S::ROW + g * (S::NARROW ? 8 : 16);
-      uint32_t odd = 0;   // bf16 pages: this lane met a value that is not finite at its i-th position
-      constexpr int MM = S::NARROW ? 1 : S::ROW / 128;
-#pragma unroll
-      for (int mm = 0; mm < MM; mm++) {
-        uint4 v[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const uint8_t *at = vp + ((i & 1) + (i >> 1) * 8) * S::ROW + mm * 128;
-          if (S::NARROW) {
-            const uint2 w = *reinterpret_cast<const uint2 *>(at);
-            v[i] = make_uint4(w.x, w.y, 0, 0);
-          } else {
-            v[i] = lds16(at);
+            for (int k = 0; k < NP; k++) {
+              const uint2 bq = qw[(k * S::KSTEPS + m * ST + j) * 32];
+              mma16816<HALF>(sc[(m * ST + j) & 3], a0, a1, a2, a3, bq.x, bq.y);
+            }
           }
         }
-        if (FMT != G4_PAGE_INT8 && !whole) {
-          // What no row sees may be anything, and 0 times an infinity or a NaN is NaN. e4m3 codes of
-          // stored rows are finite; in bf16 pages a row may see a position that another does not.
+      }
+      release(2 * n, sl, round);
+      advance();
+      // ---- softmax of the tile: sums 0, 1 are position g of rows 2c, 2c + 1; 2, 3 position g + 8.
+      float sa[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) sa[i] = (sc[0][i] + sc[1][i]) + (sc[2][i] + sc[3][i]);
+      float s0 = sa[0] * (ks0 * qf0), s1 = sa[1] * (ks0 * qf1), s2 = sa[2] * (ks1 * qf0), s3 = sa[3] * (ks1 * qf1);
+      bool see0 = on, see1 = on, see2 = on, see3 = on;
+      const bool whole = on && pos0 >= all_lo && pos0 + 16 <= all_hi;
+      uint32_t dead = 0;   // positions that no row of the warp sees
+      if (!whole && on) {
+        const int t0 = pos0 + g, t1 = t0 + 8;
+        see0 = t0 >= lo0 && t0 < hi0;
+        see1 = t0 >= lo1 && t0 < hi1;
+        see2 = t1 >= lo0 && t1 < hi0;
+        see3 = t1 >= lo1 && t1 < hi1;
+        const unsigned live0 = __ballot_sync(0xffffffffu, see0 || see1), live1 = __ballot_sync(0xffffffffu, see2 || see3);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          if (!((live0 >> (4 * i)) & 0xf)) dead |= 1u << i;
+          if (!((live1 >> (4 * i)) & 0xf)) dead |= 1u << (i + 8);
+        }
+      }
+      const float g0 = HALF ? __log2f(fmaxf(w0, 0x1p-100f)) : 0.0f, g1 = HALF ? __log2f(fmaxf(w1, 0x1p-100f)) : 0.0f;
+      s0 = see0 ? s0 : -INFINITY;
+      s1 = see1 ? s1 : -INFINITY;
+      s2 = see2 ? s2 : -INFINITY;
+      s3 = see3 ? s3 : -INFINITY;
+      float n0 = fmaxf(s0 + g0, s2 + g1), n1 = fmaxf(s1 + g0, s3 + g1);
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) {
+        n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
+        n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
+      }
+      n0 = fmaxf(n0, m0);
+      n1 = fmaxf(n1, m1);
+      if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
+        const float f0 = n0 > m0 ? ex2(m0 - n0) : 1.0f, f1 = n1 > m1 ? ex2(m1 - n1) : 1.0f;
+        l0 = n0 > m0 ? rescale(l0, m0 - n0) : l0;
+        l1 = n1 > m1 ? rescale(l1, m1 - n1) : l1;
+#pragma unroll
+        for (int i = 0; i < HD / 16; i++) {
+          o[i][0] *= f0;
+          o[i][1] *= f1;
+          o[i][2] *= f0;
+          o[i][3] *= f1;
+        }
+        m0 = n0;
+        m1 = n1;
+      }
+      uint32_t pw[2][NP];
+      {
+        const float bits = HALF ? kWeightBits : 0.0f;
+        const float r0 = m0 == -INFINITY ? 0.0f : m0 - bits, r1 = m1 == -INFINITY ? 0.0f : m1 - bits;
+        const float p0 = ex2(s0 - r0), p1 = ex2(s1 - r1), p2 = ex2(s2 - r0), p3 = ex2(s3 - r1);
+        l0 += p0 + p2;
+        l1 += p1 + p3;
+        uint32_t x[NP], y[NP];
+        split2<HALF, NP>(see0 ? p0 * w0 : 0.0f, see1 ? p1 * w0 : 0.0f, x);
+        split2<HALF, NP>(see2 ? p2 * w1 : 0.0f, see3 ? p3 * w1 : 0.0f, y);
+#pragma unroll
+        for (int k = 0; k < NP; k++) {
+          pw[0][k] = transpose8x8(x[k]);
+          pw[1][k] = transpose8x8(y[k]);
+        }
+      }
+      wait(&full[sl], round);
+      if (on) {
+        const uint8_t *vp = ring + sl * S::UNIT + 2 * c * S::ROW + g * (S::NARROW ? 8 : 16);
+        uint32_t odd = 0;   // bf16 pages: this lane met a value that is not finite at its i-th position
+        constexpr int MM = S::NARROW ? 1 : S::ROW / 128;
+#pragma unroll
+        for (int mm = 0; mm < MM; mm++) {
+          uint4 v[4];
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            if ((dead >> (2 * c + (i & 1) + (i >> 1) * 8)) & 1) v[i] = make_uint4(0, 0, 0, 0);
-            if constexpr (!HALF) {
-              uint32_t z[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+            const uint8_t *at = vp + ((i & 1) + (i >> 1) * 8) * S::ROW + mm * 128;
+            if (S::NARROW) {
+              const uint2 w = *reinterpret_cast<const uint2 *>(at);
+              v[i] = make_uint4(w.x, w.y, 0, 0);
+            } else {
+              v[i] = lds16(at);
+            }
+          }
+          if (FMT != G4_PAGE_INT8 && !whole) {
+            // What no row sees may be anything, and 0 times an infinity or a NaN is NaN. e4m3 codes of
+            // stored rows are finite; in bf16 pages a row may see a position that another does not.
 #pragma unroll
-              for (int k = 0; k < 4; k++) {
-                if ((z[k] & 0x7f80u) == 0x7f80u) {
-                  z[k] &= 0xffff0000u;
-                  odd |= 1u << i;
+            for (int i = 0; i < 4; i++) {
+              if ((dead >> (2 * c + (i & 1) + (i >> 1) * 8)) & 1) v[i] = make_uint4(0, 0, 0, 0);
+              if constexpr (!HALF) {
+                uint32_t z[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                  if ((z[k] & 0x7f80u) == 0x7f80u) {
+                    z[k] &= 0xffff0000u;
+                    odd |= 1u << i;
+                  }
+                  if ((z[k] & 0x7f800000u) == 0x7f800000u) {
+                    z[k] &= 0xffffu;
+                    odd |= 1u << i;
+                  }
                 }
-                if ((z[k] & 0x7f800000u) == 0x7f800000u) {
-                  z[k] &= 0xffffu;
-                  odd |= 1u << i;
-                }
+                v[i] = make_uint4(z[0], z[1], z[2], z[3]);
               }
-              v[i] = make_uint4(z[0], z[1], z[2], z[3]);
+            }
+          }
+          const uint32_t vw[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
+                                     {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
+          constexpr int WORDS = S::NARROW ? 2 : 4;
+          const int ob = mm * (HALF ? 8 : 4);
+#pragma unroll
+          for (int j = 0; j < WORDS; j++) {
+            if constexpr (HALF) {
+              // Four dimensions of the pairs (2c, 2c + 1) and (2c + 8, 2c + 9).
+              uint32_t e[2][4];
+#pragma unroll
+              for (int h = 0; h < 2; h++) {
+                const uint32_t t0 = __byte_perm(vw[2 * h][j], vw[2 * h + 1][j], 0x5140);
+                const uint32_t t1 = __byte_perm(vw[2 * h][j], vw[2 * h + 1][j], 0x7362);
+                codes4<FMT>(t0, e[h][0], e[h][1]);
+                codes4<FMT>(t1, e[h][2], e[h][3]);
+              }
+#pragma unroll
+              for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int k = 0; k < NP; k++)
+                  mma16816<HALF>(o[ob + 2 * j + i], e[0][2 * i], e[0][2 * i + 1], e[1][2 * i], e[1][2 * i + 1], pw[0][k], pw[1][k]);
+            } else {
+              const uint32_t a0 = __byte_perm(vw[0][j], vw[1][j], 0x5410), a1 = __byte_perm(vw[0][j], vw[1][j], 0x7632);
+              const uint32_t a2 = __byte_perm(vw[2][j], vw[3][j], 0x5410), a3 = __byte_perm(vw[2][j], vw[3][j], 0x7632);
+#pragma unroll
+              for (int k = 0; k < NP; k++) mma16816<HALF>(o[ob + j], a0, a1, a2, a3, pw[0][k], pw[1][k]);
             }
           }
         }
-        const uint32_t vw[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
-                                   {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
-        constexpr int WORDS = S::NARROW ? 2 : 4;
-        const int ob = mm * (HALF ? 8 : 4);
+        if (!HALF && __any_sync(0xffffffffu, odd != 0)) {
+          // Rows that see such a position are not finite.
+          uint32_t lanes[4];
 #pragma unroll
-        for (int j = 0; j < WORDS; j++) {
-          if constexpr (HALF) {
-            // Four dimensions of the pairs (2c, 2c + 1) and (2c + 8, 2c + 9).
-            uint32_t e[2][4];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-              const uint32_t t0 = __byte_perm(vw[2 * h][j], vw[2 * h + 1][j], 0x5140);
-              const uint32_t t1 = __byte_perm(vw[2 * h][j], vw[2 * h + 1][j], 0x7362);
-              codes4<FMT>(t0, e[h][0], e[h][1]);
-              codes4<FMT>(t1, e[h][2], e[h][3]);
-            }
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-              for (int k = 0; k < NP; k++)
-                mma16816<HALF>(o[ob + 2 * j + i], e[0][2 * i], e[0][2 * i + 1], e[1][2 * i], e[1][2 * i + 1], pw[0][k], pw[1][k]);
-          } else {
-            const uint32_t a0 = __byte_perm(vw[0][j], vw[1][j], 0x5410), a1 = __byte_perm(vw[0][j], vw[1][j], 0x7632);
-            const uint32_t a2 = __byte_perm(vw[2][j], vw[3][j], 0x5410), a3 = __byte_perm(vw[2][j], vw[3][j], 0x7632);
-#pragma unroll
-            for (int k = 0; k < NP; k++) mma16816<HALF>(o[ob + j], a0, a1, a2, a3, pw[0][k], pw[1][k]);
-          }
+          for (int i = 0; i < 4; i++) lanes[i] = __ballot_sync(0xffffffffu, (odd >> i) & 1);
+          const uint32_t of = 0x11111111u << (g >> 1);
+          const bool b0 = ((g & 1) ? lanes[1] : lanes[0]) & of, b1 = ((g & 1) ? lanes[3] : lanes[2]) & of;
+          const float nan = __int_as_float(0x7fffffff);
+          if ((b0 && see0) || (b1 && see2)) l0 = nan;
+          if ((b0 && see1) || (b1 && see3)) l1 = nan;
         }
       }
-      if (!HALF && __any_sync(0xffffffffu, odd != 0)) {
-        // Rows that see such a position are not finite.
-        uint32_t lanes[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) lanes[i] = __ballot_sync(0xffffffffu, (odd >> i) & 1);
-        const uint32_t of = 0x11111111u << (g >> 1);
-        const bool b0 = ((g & 1) ? lanes[1] : lanes[0]) & of, b1 = ((g & 1) ? lanes[3] : lanes[2]) & of;
-        const float nan = __int_as_float(0x7fffffff);
-        if ((b0 && see0) || (b1 && see2)) l0 = nan;
-        if ((b0 && see1) || (b1 && see3)) l1 = nan;
-      }
+      release(2 * n + 1, sl, round);
+      advance();
     }
-    release(2 * n + 1, sl, round);
-    advance();
-  }
-  if (bad) {
-    paged_raise(a.err, G4_PAGED_TIMEOUT);
-    // What was asked for has landed, or a second limit has passed, before the ring is given up.
-    for (int u = 2 * mine > D ? 2 * mine - D : 0; u < 2 * mine; u++) mbar_wait(&full[(ubase + u) % D], (uint32_t)(((ubase + u) / D) & 1));
-  }
+    if (bad) {
+      paged_raise(a.err, G4_PAGED_TIMEOUT);
+      // What was asked for has landed, or a second limit has passed, before the ring is given up.
+      for (int u = 2 * mine > D ? 2 * mine - D : 0; u < 2 * mine; u++) mbar_wait(&full[(ubase + u) % D], (uint32_t)(((ubase + u) / D) & 1));
+    }
 
-  // ---- join the token groups through shared memory (over Q), then write out or leave a partial.
+    // ---- join the token groups through shared memory (over Q), then write out or leave a partial.
 #pragma unroll
-  for (int x = 4; x < 32; x <<= 1) {
-    l0 += __shfl_xor_sync(0xffffffffu, l0, x);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, x);
-  }
-  __syncthreads();
-  // Partials [TG]: o [ROWS][HD], m [ROWS], l [ROWS].
-  constexpr int PART = ROWS * (HD + 2);
-  float *sm = reinterpret_cast<float *>(dsm) + tg * PART;
-#pragma unroll
-  for (int q = 0; q < HD / 16; q++) {
-    // Accumulator q: dimensions 16 g + 2 j of a 128-byte column (8 bit; 8 g + 2 j narrow or at 16 bits) and the next.
-    constexpr int PER = S::NARROW ? 4 : (HALF ? 8 : 4);
-    const int chunk = q / PER, j = q % PER;
-    const int d = chunk * (HALF && !S::NARROW ? 128 : 64) + g * (HALF && !S::NARROW ? 16 : 8) + 2 * j;
-    *reinterpret_cast<float2 *>(sm + (rt * 8 + 2 * c) * HD + d) = make_float2(o[q][0], o[q][2]);
-    *reinterpret_cast<float2 *>(sm + (rt * 8 + 2 * c + 1) * HD + d) = make_float2(o[q][1], o[q][3]);
-  }
-  if (g == 0) {
-    sm[ROWS * HD + rt * 8 + 2 * c] = m0;
-    sm[ROWS * HD + rt * 8 + 2 * c + 1] = m1;
-    sm[ROWS * HD + ROWS + rt * 8 + 2 * c] = l0;
-    sm[ROWS * HD + ROWS + rt * 8 + 2 * c + 1] = l1;
-  }
-  __syncthreads();
-  const float bits = HALF ? kWeightBits : 0.0f;
-  // Partial slots: 2 i for a part that block i begins inside of, 2 i + 1 for one it begins and leaves.
-  const int c_first = (int)((item_at + begin) / share), c_last = (int)((item_at + tiles - 1) / share), me = blockIdx.x;
-  auto slot_of = [&](int i) { return i == c_first ? 2 * i + 1 : 2 * i; };
-  float *mine_part = complete ? nullptr : a.part + (long long)slot_of(me) * PART;
-  {
-    // The same join as between blocks, its partials in shared memory.
-    const float *sp = reinterpret_cast<const float *>(dsm);
-    for (int r = t; r < ROWS; r += kDecWarps * 32) {
-      float M = -INFINITY, l = 0.0f;
-      for (int i = 0; i < TG; i++) M = fmaxf(M, sp[i * PART + ROWS * HD + r]);
-      for (int i = 0; i < TG; i++) {
-        const float m = sp[i * PART + ROWS * HD + r];
-        fsh[i * ROWS + r] = M == -INFINITY ? 0.0f : ex2(m - M);
-        l += rescale(sp[i * PART + ROWS * HD + ROWS + r], M == -INFINITY ? 0.0f : m - M);
-      }
-      fsh[TG * ROWS + r] = l;
-      const int rr = row0 + r, i = rr / a.group;
-      if (mine_part) {
-        mine_part[ROWS * HD + r] = M;
-        mine_part[ROWS * HD + ROWS + r] = l;
-      } else if (a.lse && rr < R) {
-        a.lse[(long long)(s.row + i) * a.heads + kvh * a.group + rr % a.group] =
-            M == -INFINITY ? -INFINITY : (M - bits + log2f(l)) * kLn2;
-      }
+    for (int x = 4; x < 32; x <<= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, x);
     }
     __syncthreads();
-    for (int e = t; e < ROWS * (HD / 4); e += kDecWarps * 32) {
-      const int r = e / (HD / 4), d = e % (HD / 4) * 4, rr = row0 + r, i = rr / a.group;
-      float4 v = make_float4(0, 0, 0, 0);
+    // Partials [TG]: o [ROWS][HD], m [ROWS], l [ROWS].
+    constexpr int PART = ROWS * (HD + 2);
+    float *sm = reinterpret_cast<float *>(dsm) + tg * PART;
 #pragma unroll
-      for (int k = 0; k < TG; k++) {
-        const float f = fsh[k * ROWS + r];
-        const float4 z = *reinterpret_cast<const float4 *>(sp + k * PART + r * HD + d);
-        v.x = fmaf(f, z.x, v.x);
-        v.y = fmaf(f, z.y, v.y);
-        v.z = fmaf(f, z.z, v.z);
-        v.w = fmaf(f, z.w, v.w);
-      }
-      if (mine_part) {
-        *reinterpret_cast<float4 *>(mine_part + r * HD + d) = v;
-        continue;
-      }
-      if (rr >= R) continue;
-      const float l = fsh[TG * ROWS + r], inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-      const long long at = (long long)(s.row + i) * a.o_stride + (long long)(kvh * a.group + rr % a.group) * HD + d;
-      if (a.type == G4_F32) {
-        *reinterpret_cast<float4 *>((float *)a.out + at) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-      } else {
-        *reinterpret_cast<uint2 *>((__nv_bfloat16 *)a.out + at) = make_uint2(
-            [&] { const __nv_bfloat162 h = __floats2bfloat162_rn(v.x * inv, v.y * inv); return *reinterpret_cast<const uint32_t *>(&h); }(),
-            [&] { const __nv_bfloat162 h = __floats2bfloat162_rn(v.z * inv, v.w * inv); return *reinterpret_cast<const uint32_t *>(&h); }());
-      }
+    for (int q = 0; q < HD / 16; q++) {
+      // Accumulator q: dimensions 16 g + 2 j of a 128-byte column (8 bit; 8 g + 2 j narrow or at 16 bits) and the next.
+      constexpr int PER = S::NARROW ? 4 : (HALF ? 8 : 4);
+      const int chunk = q / PER, j = q % PER;
+      const int d = chunk * (HALF && !S::NARROW ? 128 : 64) + g * (HALF && !S::NARROW ? 16 : 8) + 2 * j;
+      *reinterpret_cast<float2 *>(sm + (rt * 8 + 2 * c) * HD + d) = make_float2(o[q][0], o[q][2]);
+      *reinterpret_cast<float2 *>(sm + (rt * 8 + 2 * c + 1) * HD + d) = make_float2(o[q][1], o[q][3]);
     }
-  }
-  if (!complete) {
-    // ---- the last of each kJoin neighbours joins them; the last of those the whole.
-    const int parts = c_last - c_first + 1, groups = (parts + kJoin - 1) / kJoin, grp = (me - c_first) / kJoin;
-    const int g0 = c_first + grp * kJoin, in_group = min(kJoin, parts - grp * kJoin);
-    uint32_t *group_count = a.count + 2 * slot_of(g0), *all_count = a.count + 2 * slot_of(c_first) + 1;
-    __syncthreads();
-    if (t == 0) {
-      __threadfence();   // (orders what the barrier has ordered before it)
-      const bool last = atomicAdd(group_count, 1u) == (unsigned)in_group - 1;
-      __threadfence();
-      if (last) *group_count = 0;
-      sum_sh[1] = last;
+    if (g == 0) {
+      sm[ROWS * HD + rt * 8 + 2 * c] = m0;
+      sm[ROWS * HD + rt * 8 + 2 * c + 1] = m1;
+      sm[ROWS * HD + ROWS + rt * 8 + 2 * c] = l0;
+      sm[ROWS * HD + ROWS + rt * 8 + 2 * c + 1] = l1;
     }
     __syncthreads();
-    if (sum_sh[1]) {
-      // Slots of a group's members are 2 PART apart from the second on; the first one's place differs.
-      float *base = a.part + (long long)slot_of(g0) * PART;
-      join_partials<HD>(a, base, in_group > 1 ? a.part + (long long)slot_of(g0 + 1) * PART : nullptr, 2ll * PART, in_group, ROWS,
-                        groups > 1 ? base : nullptr, s, kvh, row0, bits, fsh);
-      if (groups > 1) {
-        __syncthreads();
-        if (t == 0) {
-          __threadfence();
-          const bool last = atomicAdd(all_count, 1u) == (unsigned)groups - 1;
-          __threadfence();
-          if (last) *all_count = 0;
-          sum_sh[2] = last;
+    const float bits = HALF ? kWeightBits : 0.0f;
+    // Partial slots: 2 i for a part that block i begins inside of, 2 i + 1 for one it begins and leaves.
+    const int c_first = (int)((item_at + begin) / share), c_last = (int)((item_at + tiles - 1) / share), me = blockIdx.x;
+    auto slot_of = [&](int i) { return i == c_first ? 2 * i + 1 : 2 * i; };
+    float *mine_part = complete ? nullptr : a.part + (long long)slot_of(me) * PART;
+    {
+      // The same join as between blocks, its partials in shared memory.
+      const float *sp = reinterpret_cast<const float *>(dsm);
+      for (int r = t; r < ROWS; r += kDecWarps * 32) {
+        float M = -INFINITY, l = 0.0f;
+        for (int i = 0; i < TG; i++) M = fmaxf(M, sp[i * PART + ROWS * HD + r]);
+        for (int i = 0; i < TG; i++) {
+          const float m = sp[i * PART + ROWS * HD + r];
+          fsh[i * ROWS + r] = M == -INFINITY ? 0.0f : ex2(m - M);
+          l += rescale(sp[i * PART + ROWS * HD + ROWS + r], M == -INFINITY ? 0.0f : m - M);
         }
-        __syncthreads();
-        if (sum_sh[2]) {
-          join_partials<HD>(a, a.part + (long long)slot_of(c_first) * PART, a.part + (long long)slot_of(c_first + kJoin) * PART,
-                            2ll * kJoin * PART, groups, ROWS, nullptr, s, kvh, row0, bits, fsh);
+        fsh[TG * ROWS + r] = l;
+        const int rr = row0 + r, i = rr / a.group;
+        if (mine_part) {
+          mine_part[ROWS * HD + r] = M;
+          mine_part[ROWS * HD + ROWS + r] = l;
+        } else if (a.lse && rr < R) {
+          a.lse[(long long)(s.row + i) * a.heads + kvh * a.group + rr % a.group] =
+              M == -INFINITY ? -INFINITY : (M - bits + log2f(l)) * kLn2;
+        }
+      }
+      __syncthreads();
+      for (int e = t; e < ROWS * (HD / 4); e += kDecWarps * 32) {
+        const int r = e / (HD / 4), d = e % (HD / 4) * 4, rr = row0 + r, i = rr / a.group;
+        float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < TG; k++) {
+          const float f = fsh[k * ROWS + r];
+          const float4 z = *reinterpret_cast<const float4 *>(sp + k * PART + r * HD + d);
+          v.x = fmaf(f, z.x, v.x);
+          v.y = fmaf(f, z.y, v.y);
+          v.z = fmaf(f, z.z, v.z);
+          v.w = fmaf(f, z.w, v.w);
+        }
+        if (mine_part) {
+          *reinterpret_cast<float4 *>(mine_part + r * HD + d) = v;
+          continue;
+        }
+        if (rr >= R) continue;
+        const float l = fsh[TG * ROWS + r], inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        const long long at = (long long)(s.row + i) * a.o_stride + (long long)(kvh * a.group + rr % a.group) * HD + d;
+        if (a.type == G4_F32) {
+          *reinterpret_cast<float4 *>((float *)a.out + at) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        } else {
+          *reinterpret_cast<uint2 *>((__nv_bfloat16 *)a.out + at) = make_uint2(
+              [&] { const __nv_bfloat162 h = __floats2bfloat162_rn(v.x * inv, v.y * inv); return *reinterpret_cast<const uint32_t *>(&h); }(),
+              [&] { const __nv_bfloat162 h = __floats2bfloat162_rn(v.z * inv, v.w * inv); return *reinterpret_cast<const uint32_t *>(&h); }());
         }
       }
     }
-  }
-  ubase += 2 * mine;
-  at += count;
-  if (at < end) {
-    // The next part's positions come over what this one's partials took up.
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncthreads();
-  }
+    if (!complete) {
+      // ---- the last of each kJoin neighbours joins them; the last of those the whole.
+      const int parts = c_last - c_first + 1, groups = (parts + kJoin - 1) / kJoin, grp = (me - c_first) / kJoin;
+      const int g0 = c_first + grp * kJoin, in_group = min(kJoin, parts - grp * kJoin);
+      uint32_t *group_count = a.count + 2 * slot_of(g0), *all_count = a.count + 2 * slot_of(c_first) + 1;
+      __syncthreads();
+      if (t == 0) {
+        __threadfence();   // (orders what the barrier has ordered before it)
+        const bool last = atomicAdd(group_count, 1u) == (unsigned)in_group - 1;
+        __threadfence();
+        if (last) *group_count = 0;
+        sum_sh[1] = last;
+      }
+      __syncthreads();
+      if (sum_sh[1]) {
+        // Slots of a group's members are 2 PART apart from the second on; the first one's place differs.
+        float *base = a.part + (long long)slot_of(g0) * PART;
+        join_partials<HD>(a, base, in_group > 1 ? a.part + (long long)slot_of(g0 + 1) * PART : nullptr, 2ll * PART, in_group, ROWS,
+                          groups > 1 ? base : nullptr, s, kvh, row0, bits, fsh);
+        if (groups > 1) {
+          __syncthreads();
+          if (t == 0) {
+            __threadfence();
+            const bool last = atomicAdd(all_count, 1u) == (unsigned)groups - 1;
+            __threadfence();
+            if (last) *all_count = 0;
+            sum_sh[2] = last;
+          }
+          __syncthreads();
+          if (sum_sh[2]) {
+            join_partials<HD>(a, a.part + (long long)slot_of(c_first) * PART, a.part + (long long)slot_of(c_first + kJoin) * PART,
+                              2ll * kJoin * PART, groups, ROWS, nullptr, s, kvh, row0, bits, fsh);
+          }
+        }
+      }
+    }
+    ubase += 2 * mine;
+    at += count;
+    if (at < end) {
+      // The next part's positions come over what this one's partials took up.
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncthreads();
+    }
   }
 }
 
@@ -848,13 +848,12 @@ static int decode_rt(const PagedAttn &a) {
 
 static_assert(4 * 148 * 4 <= kPagedCounters, "two counters a partial, two partials a block");
 
-// Tiles a warp group works on before a share is split further.
 static void plan_decode(PagedAttn &a) {
   const int rt = decode_rt(a), rows = 8 * rt;
   a.row_groups = (int)(((long long)a.max_q * a.group + rows - 1) / rows);
-  a.split_tiles = SPLIT_T * kDecWarps / rt;
+  a.split_tiles = kLeastTiles * kDecWarps / rt;
   // (One context alone: no share holds a second beginning.)
-  a.begin_tiles = (long long)a.batch * a.pool.kv_heads * a.row_groups == 1 ? 1 : BEGIN_T;
+  a.begin_tiles = (long long)a.batch * a.pool.kv_heads * a.row_groups == 1 ? 1 : kBeginTiles;
 }
 
 size_t paged_attention_partials(const PagedAttn &args) {

@@ -262,7 +262,14 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
     first = lo >> 4;
     return (hi > lo ? ((hi + 15) >> 4) - first : 0) + a.begin_tiles;
   };
-  // All tiles of sequence b.
+  // All row groups' tiles of a sequence for one KV head, by the whole warp.
+  auto all_groups = [&](const SeqSpan &s) {
+    int n = 0, first;
+    if (a.row_groups == 1) return tiles_of(s, 0, first);
+    for (int rg = lane; rg < a.row_groups; rg += 32) n += tiles_of(s, rg, first);
+    return __reduce_add_sync(0xffffffffu, n);
+  };
+  // All tiles of sequence b, by one thread.
   auto seq_tiles = [&](int b, bool report) -> long long {
     const SeqSpan s = seq_span(a, b, report);
     int n = 0, first;
@@ -272,9 +279,16 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
   // Thread t holds the tiles of its share of the sequences; the block's scan gives where each begins.
   const int per = (a.batch + NT - 1) / NT;
   long long mine_sum = 0;
-  for (int i = 0; i < per; i++) {
-    const int b = t * per + i;
-    if (b < a.batch) mine_sum += seq_tiles(b, blockIdx.x == 0);
+  if (a.row_groups < 8) {
+    for (int i = 0; i < per; i++) {
+      const int b = t * per + i;
+      if (b < a.batch) mine_sum += seq_tiles(b, blockIdx.x == 0);
+    }
+  } else {   // (a chunk of f32 rows has hundreds: a sequence at a time, 32 groups at once)
+    for (int b = warp * 32 * per; b < min(a.batch, (warp + 1) * 32 * per); b++) {
+      const int n = all_groups(seq_span(a, b, blockIdx.x == 0 && lane == 0));
+      if (lane == b / per - warp * 32) mine_sum += (long long)n * p.kv_heads;
+    }
   }
   long long incl = mine_sum;
 #pragma unroll
@@ -328,8 +342,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
     int kvh = 0, rg = 0, first = 0, tiles;
     long long item_at = seq_at;
     {
-      int all = 0;
-      for (int r = 0; r < a.row_groups; r++) all += tiles_of(s, r, first);
+      const int all = all_groups(s);
       if (at >= seq_at + (long long)all * p.kv_heads) {   // this sequence is done
         seq_at += (long long)all * p.kv_heads;
         b++;
@@ -337,11 +350,30 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
       }
       kvh = (int)((at - seq_at) / all);
       item_at += (long long)kvh * all;
-      tiles = tiles_of(s, 0, first);
-      while (at >= item_at + tiles) {
-        item_at += tiles;
-        tiles = tiles_of(s, ++rg, first);
+      if (a.row_groups > 1) {
+        // The row group that `at` lies in: a scan of 32 at a time.
+        int off = (int)(at - item_at), unused;
+        for (int r0 = 0;; r0 += 32) {
+          const int n = r0 + lane < a.row_groups ? tiles_of(s, r0 + lane, unused) : 0;
+          int upto = n;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += o;
+          }
+          const unsigned past = __ballot_sync(0xffffffffu, off < upto);
+          if (past) {
+            const int l = __ffs((int)past) - 1;
+            rg = r0 + l;
+            item_at += __shfl_sync(0xffffffffu, upto - n, l);
+            break;
+          }
+          const int sum = __shfl_sync(0xffffffffu, upto, 31);
+          off -= sum;
+          item_at += sum;
+        }
       }
+      tiles = tiles_of(s, rg, first);
     }
     const int R = s.n * a.group, row0 = rg * ROWS;
     const int from = (int)(at - item_at), count = (int)min((long long)tiles - from, end - at);

@@ -365,7 +365,7 @@ int check_attention(const char *who, const g4_page_pool *pool, int32_t type, int
     return set_error(G4_ERR_UNSUPPORTED, "%s: rows %d x %d heads (fewer than 2^30), batch %d (at most 65535), max_kv %d (2^30)", who, rows, heads, batch, max_kv);
   // A sequence's tiles (16 positions x up to 32 rows) are counted in 32 bits.
   const long long q_rows = (long long)(max_q < rows ? max_q : rows) * (heads / a->pool.kv_heads);
-  if ((type == G4_F32 || q_rows <= 32) && ((long long)max_kv / 16 + 32) * (q_rows / 32 + 1) >= (1ll << 31))
+  if ((type == G4_F32 || max_kv > (1 << 24) || q_rows <= 32) && ((long long)max_kv / 16 + 32) * (q_rows / 32 + 1) >= (1ll << 31))
     return set_error(G4_ERR_UNSUPPORTED, "%s: %lld rows over %d positions in one sequence", who, q_rows, max_kv);
   a->type = type;
   a->heads = heads;

@@ -869,8 +869,27 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<FMT, HD, NP, RT>::OCC
 }
 
 // ------------------------------------------------------------------------------ launch
-// More rows per KV head than a block here holds: the chunk kernel's 128-row tiles.
-static bool chunk_path(const PagedAttn &a) { return a.type == G4_BF16 && (long long)a.max_q * a.group > 32; }
+// Whether the chunk kernel takes the call. Its blocks own 128 rows and walk their context alone, so its time
+// is that walk (about 2.4 us a block of 128 positions at head_dim 256, and 10) times its rounds over the
+// SMs; here the list is spread over all SMs but costs the more the more rows it has (about 45 us and
+// 6.5 ns a tile of 16 positions x 32 rows). Both in us, from (B x new tokens of 8 heads over a
+// context: chunk, here) 64 x 8 over 2,000: 56, 142; 64 x 3: 55, 84; 16 x 8: 51, 63; 1 x 8 over 8,000: 153, 54;
+// 1 x 32: 155, 74; 8 x 32: 156, 234. Up to 16 rows the padding of a 128-row tile does not pay; f32 rows need
+// products in parts, which only the kernel here carries.
+static bool chunk_path(const PagedAttn &a) {
+  const long long rows = (long long)a.max_q * a.group;
+  if (a.type != G4_BF16 || rows <= 16) return false;
+  const int hd = a.pool.hd, tokens = 128 / a.group;
+  const double walk = hd == 512 ? 1.45 : (hd == 256 ? 1.0 : (hd == 128 ? 0.8 : 0.7));
+  const double tile = hd == 512 ? 2.0 : (hd == 256 ? 1.0 : (hd == 128 ? 0.75 : 0.65));
+  double span = a.max_kv;
+  if (a.window > 0) span = std::min(span, (double)a.window + std::min(a.max_q, tokens));
+  const long long heads = (long long)a.batch * a.pool.kv_heads;
+  const long long blocks = heads * ((a.max_q + tokens - 1) / tokens) * (hd == 512 ? 2 : 1);
+  const double chunk = (double)((blocks + 147) / 148) * (10.0 + 2.4 * walk * (span / 128 + 1));
+  const double list = 45.0 + 0.0065 * tile * (double)(heads * ((rows + 31) / 32)) * (span / 16);
+  return chunk < list;
+}
 
 // Row tiles per block: 1 for a group's 8 rows, up to 4 (each reads the positions again, from L1).
 static int decode_rt(const PagedAttn &a) {

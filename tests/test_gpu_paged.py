@@ -661,3 +661,29 @@ def test_bf16_values_a_row_does_not_see_never_reach_it(paged, cuda, q_len, bad):
     out = paged.attention(pool, q, *args, scale=0.05)
     assert torch.equal(out[:-1], good[:-1])
     assert not out[-1, :, 5].isfinite().any()
+
+
+@pytest.mark.parametrize("fmt,page,q_len", [("bf16", 1024, 1), ("bf16", 1024, 40), ("int8", 1024, 1), ("int8", 1024, 40)])
+def test_offsets_past_32_bits(paged, cuda, fmt, page, q_len):
+    """The last pages of a pool of more than 2^32 bytes (and 2^31 values) give what the same rows give in
+    a small pool, bit for bit."""
+    torch = cuda
+    heads, hd = 8, 512
+    pages = (2 ** 32 // (heads * page * hd * (2 if fmt == "bf16" else 1))) + 3
+    big = paged.PagePool.create(pages, page, heads, hd, fmt)
+    small = paged.PagePool.create(2, page, heads, hd, fmt)
+    kv = page + 300
+    k = torch.randn(kv, heads, hd, generator=gen(torch, 1), device="cuda").bfloat16()
+    v = torch.randn(kv, heads, hd, generator=gen(torch, 2), device="cuda").bfloat16()
+    q = torch.randn(q_len, 2 * heads, hd, generator=gen(torch, 3), device="cuda").bfloat16()
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    outs = []
+    for pool, ids in ((big, [pages - 1, pages - 2]), (small, [1, 0])):
+        slots = torch.tensor([ids[t // page] * page + t % page for t in range(kv)], dtype=torch.int32, device="cuda")
+        pool.store(k, v, slots)
+        out = paged.attention(pool, q, ints([0, q_len]), ints([kv - q_len]), ints([kv]), ints([ids]), q_len, kv, scale=0.04)
+        outs.append((out, *pool.read(slots, torch.bfloat16)))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    assert outs[0][0].float().abs().max() > 0 and (outs[0][1].float() - k.float()).abs().max() < 0.05
+    del big
+    torch.cuda.empty_cache()

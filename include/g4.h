@@ -478,7 +478,8 @@ int g4_op_page_read(const g4_page_pool *pool, const int32_t *slots, int32_t toke
  * not read.
  *   out = sum_t softmax_t(scale * q . k_t) v_t, lse = ln sum_t exp(scale * q . k_t)
  * with lse f32 [rows, heads] or NULL. A row that sees nothing gets out 0 and lse -inf. Values at
- * positions that a row does not see never reach it, whatever they are. max_q and max_kv bound the
+ * positions that a row does not see never reach it, whatever they are; a row that sees a K or V
+ * value that is not finite is not finite where it enters, and may be NaN throughout. max_q and max_kv bound the
  * sequences' rows and kv_len: a longer sequence, rows past `rows` or positions past the page table
  * are cut off there and raise G4_PAGED_BAD_LENGTH; a page outside the pool is left out and raises
  * G4_PAGED_BAD_PAGE. Sums and softmax statistics are f32 and in a fixed order: results do not
